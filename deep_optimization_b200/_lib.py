@@ -21,7 +21,8 @@ ACT_FLAG_META_BF16 = 16
 ACT_FLAG_BALLOT_REF_BIAS = 32
 ACT_GEMM_B_IS_NK = 1
 ACT_GEMM_SINGLE_CTA = 2
-ACT_KIND_GELU, ACT_KIND_SILU, ACT_KIND_GELU_ERF = 1, 2, 3
+ACT_KIND_NONE, ACT_KIND_GELU, ACT_KIND_SILU, ACT_KIND_GELU_ERF, ACT_KIND_RELU = 0, 1, 2, 3, 4
+ACT_LINEAR_PAIR, ACT_LINEAR_128, ACT_LINEAR_64, ACT_LINEAR_FEW_ROWS = 1, 2, 3, 4
 
 # every symbol include/act_b200.h declares, with its ctypes signature
 _vp, _i32, _i64, _u64, _f32 = (ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64,
@@ -76,6 +77,19 @@ SIGNATURES = {
     "act_ln_bwd_from_packed_sum": ([_vp, _vp, _i32, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
                                     _vp], _i32),
     "act_merge_heads": ([_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp], _i32),
+    "act_linear_fwd_workspace": ([_vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32], _sz),
+    "act_linear_fwd": ([_vp, _i64, _vp, _i64, _vp, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _i32,
+                        _vp, _sz, _vp], _i32),
+    "act_mul_col_sum_workspace": ([_i64, _i32], _sz),
+    "act_mul_col_sum": ([_vp, _vp, _i32, _i64, _i32, _vp, _vp, _vp, _sz, _vp], _i32),
+    "act_linear_bwd_workspace": ([_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32], _sz),
+    "act_linear_bwd": ([_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _sz,
+                        _vp], _i32),
+    "act_linear_status": ([_vp, _i32], _i32),
+    "act_dropout": ([_vp, _vp, _i32, _i64, ctypes.c_uint, _u64, _u64, _vp, _vp, _vp], _i32),
+    "act_rng_ticket": ([_vp, _vp, _vp], _i32),
+    "act_rotary_heads": ([_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i64, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _i32, _i32,
+                          _i32, _vp], _i32),
     "act_calc_precision": ([_vp, _vp, _vp, _i64, ctypes.c_double], _i32),
     "act_fp8_gemm_workspace": ([_i32, _i32, _i32, _i32], ctypes.c_size_t),
     "act_fp8_gemm": ([_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, ctypes.c_size_t, _vp], _i32),

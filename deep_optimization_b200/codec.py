@@ -846,3 +846,89 @@ def ln_bwd_from_packed(dy: torch.Tensor, packed: torch.Tensor, scale: torch.Tens
             None if w is None else w.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), _stream_ptr(dy))
     _lib.check(rc, "act_ln_bwd_from_packed_sum")
     return dx, dgamma, dbeta
+
+
+# ---------------------------------------------------------------- dropout without a stored mask
+
+# {device index: [seed of the stream, int64 [2] on the device: seed and next number]}, for launches
+# inside captured graphs
+_graph_rng = {}
+
+
+def dropout_threshold(p: float) -> int:
+    """The dropping probability in 2^-16, what the kernel compares sixteen random bits with."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability has to be between 0 and 1, but got {p}")
+    return int(p * 65536.0 + 0.5)
+
+
+def dropout_rng(device):
+    """(seed, offset) for one dropout call on a CUDA device: the seed and position of PyTorch's own
+    generator of that device, which is moved on, so that `torch.manual_seed` makes a run repeatable and
+    a recomputation under `torch.utils.checkpoint` sees the mask of the first pass.  Ranks of a
+    torch.distributed job that share a seed draw different masks, as in `manual_seed`.
+
+    Inside a CUDA graph capture the pair is an int64 [2] tensor on the device instead, taken from a
+    stream that lives there, so that each replay draws a new mask; one call outside any capture has to
+    come first on each device."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    if torch.cuda.is_current_stream_capturing():
+        if index not in _graph_rng:
+            raise RuntimeError("dropout_rng: run one step outside the capture first (the device's stream of mask "
+                               "numbers is set up then)")
+        state = _graph_rng[index][1]
+        out = torch.empty(2, dtype=torch.int64, device=state.device)
+        with _device_of(out):
+            _lib.check(_lib.load().act_rng_ticket(state.data_ptr(), out.data_ptr(), _stream_ptr(out)), "act_rng_ticket")
+        return out
+    gen = torch.cuda.default_generators[index]
+    seed, offset = gen.initial_seed(), gen.get_offset()
+    gen.set_offset(offset + 4)
+    if torch.distributed.is_available() and torch.distributed.is_initialized() and torch.distributed.get_rank():
+        seed ^= _mix64(torch.distributed.get_rank())
+    seed &= 0xFFFFFFFFFFFFFFFF
+    have = _graph_rng.get(index)
+    if have is None or have[0] != seed:
+        # numbers from 2^62 on: never an offset of the generator
+        fresh = torch.tensor([seed - (1 << 64) if seed >> 63 else seed, 1 << 62], dtype=torch.int64)
+        if have is None:
+            _graph_rng[index] = [seed, fresh.to(torch.device("cuda", index))]
+        else:
+            have[0] = seed
+            have[1].copy_(fresh)
+    return seed, offset
+
+
+def dropout(x: torch.Tensor, p: float, rng, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Dropout of x with probability p, plus `residual` (x's shape and type) where given.  The mask is a
+    function of `rng`, a (seed, offset) pair or the device tensor that `dropout_rng` gives, and of the
+    element's place in memory: the gradient of x is this call on dy with the same `p` and `rng`, dy being
+    laid out as x.  p counts in 2^-16 (an element is kept when its sixteen random bits reach
+    round(65536 p)) and the kept elements' factor is that of the rounded probability.  A dropped
+    element gives 0 whatever it holds."""
+    _require_cuda(x, "x")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"unsupported activation dtype {x.dtype}")
+    t = dropout_threshold(p)
+    if not is_channels_last(x):
+        x = x.contiguous()
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+            raise ValueError("dropout: the residual must have x's shape, type and device")
+        if residual.stride() != x.stride():
+            residual = torch.empty_like(x).copy_(residual)
+    seed = offset = 0
+    rng_ptr = None
+    if isinstance(rng, torch.Tensor):
+        if rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous() or rng.device != x.device:
+            raise ValueError("dropout: rng must be a (seed, offset) pair or a contiguous int64 [2] tensor on x's device")
+        rng_ptr = rng.data_ptr()
+    else:
+        seed, offset = rng
+    y = torch.empty_like(x)
+    with _device_of(x):
+        rc = _lib.load().act_dropout(x.data_ptr(), None if residual is None else residual.data_ptr(), _DTYPES[x.dtype],
+                                     x.numel(), t, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, rng_ptr,
+                                     y.data_ptr(), _stream_ptr(x))
+    _lib.check(rc, "act_dropout")
+    return y

@@ -23,7 +23,7 @@ from torch import nn
 from torch.fx.passes.shape_prop import ShapeProp
 
 from .layers import DOConv1d, DOConv2d, DOConv3d, DODepthPointConv2d, DOLinear, RMSNorm
-from .modules.activations.act_layers import DOGELU, DOMaxPool2d, DOReLU_Variance, DOSiLU
+from .modules.activations.act_layers import DODropout, DOGELU, DOMaxPool2d, DOReLU_Variance, DOSiLU
 from .modules.normalization.normalization_layers import DOBatchNorm2d, DOLayerNorm, DOSyncBatchNorm2d
 from .quantizer import Quantizer
 
@@ -359,6 +359,12 @@ class Controller:
                         setattr(traced.get_submodule(parent_path), child,
                                 DOMaxPool2d(mod.kernel_size, mod.stride, mod.padding, mod.dilation,
                                             mod.return_indices, mod.ceil_mode))
+            if self.config.get("compress_dropout", False):
+                # an extension, on request only: the masks come from another generator than PyTorch's
+                for name, mod in list(traced.named_modules()):
+                    if type(mod) is nn.Dropout:
+                        parent_path, _, child = name.rpartition(".")
+                        setattr(traced.get_submodule(parent_path), child, DODropout(mod.p))
             self.fused_add_layer_norm = []
             if self.config.get("fuse_add_layer_norm", True):
                 self.fused_add_layer_norm = self._fuse_add_layer_norm(traced)

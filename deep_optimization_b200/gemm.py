@@ -105,3 +105,165 @@ def dw_status(clear: bool = True) -> int:
     v = ctypes.c_uint(0)
     _lib.check(_lib.load().act_dw_from_packed_status(ctypes.byref(v), 1 if clear else 0), "act_dw_from_packed_status")
     return int(v.value)
+
+
+# ---------------------------------------------------------------- linear with its epilogue
+
+_ACTIVATIONS = {"none": _lib.ACT_KIND_NONE, "relu": _lib.ACT_KIND_RELU, "gelu": _lib.ACT_KIND_GELU,
+                "gelu_erf": _lib.ACT_KIND_GELU_ERF, "silu": _lib.ACT_KIND_SILU}
+_DTYPE16 = {torch.bfloat16: _lib.ACT_DTYPE_BF16, torch.float16: _lib.ACT_DTYPE_F16}
+_DTYPES = {torch.float32: _lib.ACT_DTYPE_F32, **_DTYPE16}
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t as a matrix of its last dimension whose rows are contiguous and do not overlap."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+        t = t.contiguous()
+    return t
+
+
+def _pitch(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def linear_act_applies(x: torch.Tensor, weight: torch.Tensor) -> bool:
+    """linear_act takes bf16 or fp16 CUDA tensors of one type and device, at least one input feature."""
+    return (x.is_cuda and x.dtype in _DTYPE16 and weight.dtype == x.dtype and weight.device == x.device
+            and weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1] > 0)
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
+               residual: Optional[torch.Tensor] = None, derivative: bool = False, variant: int = 0):
+    """y = f(x @ weight.T + bias) + residual in one kernel (the sum in fp32, rounded once), for bf16 or fp16
+    x [..., K] and weight [N, K] of the same type; bias [N] bf16, fp16 or fp32; residual [..., N] of x's type.
+    `activation`: "none", "relu", "gelu" (tanh form), "gelu_erf" or "silu".  With `derivative` (GELU and SiLU)
+    the result is (y, f'(...)): what a layer that saves the derivative, not its input, keeps for backward.
+    Without autograd; `layers.DOLinearAct` is the module.  `variant` names a kernel (ACT_LINEAR_*) instead of
+    the library's own choice."""
+    if not x.is_cuda:
+        raise RuntimeError("linear_act needs CUDA tensors: there is no CPU path")
+    dt = _DTYPE16.get(x.dtype)
+    if dt is None or weight.dtype != x.dtype:
+        raise TypeError(f"linear_act: x and weight must both be bfloat16 or both float16, got {x.dtype} and {weight.dtype}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"linear_act: activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+    if derivative and activation in ("none", "relu"):
+        raise ValueError("linear_act: the derivative is an output of the GELU and SiLU forms only")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.shape[1] == 0:
+        raise ValueError(f"linear_act: x [..., K] and weight [N, K] with K > 0, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    N, K = weight.shape
+    shape = x.shape[:-1] + (N,)
+    bias_dt = 0
+    if bias is not None:
+        if bias.shape != (N,) or bias.dtype not in _DTYPES or bias.device != x.device:
+            raise ValueError("linear_act: bias must be [N], of a floating type of 16 or 32 bits, on x's device")
+        bias = bias.contiguous()
+        bias_dt = _DTYPES[bias.dtype]
+    if weight.device != x.device:
+        raise ValueError("linear_act: weight must be on x's device")
+    x2, w2, r2 = _rows(x), _rows(weight), None
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != x.dtype or residual.device != x.device:
+            raise ValueError(f"linear_act: residual must have the result's shape {tuple(shape)}, type and device")
+        r2 = _rows(residual)
+    M = x2.shape[0]
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    d = torch.empty_like(y) if derivative else None
+    lib = _lib.load()
+    xp, wp, ldx, ldw = x2.data_ptr(), w2.data_ptr(), _pitch(x2), _pitch(w2)
+    ws_ptr = ws = None
+    need = lib.act_linear_fwd_workspace(xp, ldx, wp, ldw, M, N, K, variant)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        ws_ptr = ws.data_ptr()
+    with _lib.device_of(x):
+        rc = lib.act_linear_fwd(xp, ldx, wp, ldw, None if bias is None else bias.data_ptr(), bias_dt,
+                                None if r2 is None else r2.data_ptr(), 0 if r2 is None else _pitch(r2), dt, M, N, K,
+                                _ACTIVATIONS[activation], y.data_ptr(), N, None if d is None else d.data_ptr(), N, variant,
+                                ws_ptr, need, _lib.stream_ptr(x))
+    _lib.check(rc, "act_linear_fwd")
+    return (y, d) if derivative else y
+
+
+def act_backward(dy: torch.Tensor, derivative: torch.Tensor, bias_grad: bool = True):
+    """(dz, db) of z -> f(z) with f'(z) = `derivative`: dz = dy * derivative in their type and, with
+    `bias_grad`, db = its sum over everything but the last dimension, fp32, of the products before that
+    rounding; None otherwise.  bf16 or fp16, one pass; the sum's order is fixed."""
+    if not dy.is_cuda:
+        raise RuntimeError("act_backward needs CUDA tensors: there is no CPU path")
+    if dy.dtype not in _DTYPE16 or derivative.dtype != dy.dtype:
+        raise TypeError("act_backward: dy and derivative must both be bfloat16 or both float16")
+    if derivative.shape != dy.shape or dy.dim() < 1 or derivative.device != dy.device:
+        raise ValueError("act_backward: dy and derivative must have one shape and device")
+    dy, derivative = dy.contiguous(), derivative.contiguous()
+    N = dy.shape[-1]
+    M = dy.numel() // N if N else 0
+    dz = torch.empty_like(dy)
+    lib = _lib.load()
+    db = ws = None
+    need = 0
+    if bias_grad:
+        db = torch.empty(N, dtype=torch.float32, device=dy.device)
+        need = lib.act_mul_col_sum_workspace(M, N)
+        ws = torch.empty(need, dtype=torch.uint8, device=dy.device)
+    with _lib.device_of(dy):
+        rc = lib.act_mul_col_sum(dy.data_ptr(), derivative.data_ptr(), _DTYPE16[dy.dtype], M, N, dz.data_ptr(),
+                                 None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), need,
+                                 _lib.stream_ptr(dy))
+    _lib.check(rc, "act_mul_col_sum")
+    return dz, db
+
+
+def linear_backward(dz: torch.Tensor, x: Optional[torch.Tensor], weight: Optional[torch.Tensor], need_dx: bool = True,
+                    need_dw: bool = True, dw_dtype: Optional[torch.dtype] = None, variant: int = 0):
+    """(dx, dw) of z = x @ weight.T from dz [..., N]: dx = dz @ weight and dw = dz.T @ x over all rows, in dz's
+    type (dw in float32 if `dw_dtype` says so), None where not needed (x or weight may then be None).
+    bf16 or fp16, sums in fp32; dw's long reduction is split over the GPU and joined in a fixed order."""
+    if not dz.is_cuda:
+        raise RuntimeError("linear_backward needs CUDA tensors: there is no CPU path")
+    dt = _DTYPE16.get(dz.dtype)
+    x = x if need_dw else None
+    weight = weight if need_dx else None
+    if dt is None or any(t is not None and t.dtype != dz.dtype for t in (x, weight)):
+        raise TypeError("linear_backward: dz, x and weight must all be bfloat16 or all float16")
+    dw_dtype = dz.dtype if dw_dtype is None else dw_dtype
+    if dw_dtype not in (dz.dtype, torch.float32):
+        raise TypeError("linear_backward: dw comes in dz's type or in float32")
+    if dz.dim() < 1 or (need_dw and (x is None or x.shape[:-1] != dz.shape[:-1])) \
+            or (need_dx and (weight is None or weight.dim() != 2 or weight.shape[0] != dz.shape[-1])) \
+            or any(t is not None and t.device != dz.device for t in (x, weight)) \
+            or (need_dx and need_dw and x.shape[-1] != weight.shape[1]):
+        raise ValueError("linear_backward: dz [..., N], x [..., K] and weight [N, K] on one device")
+    if not need_dx and not need_dw:
+        return None, None
+    N = dz.shape[-1]
+    K = weight.shape[1] if need_dx else x.shape[-1]
+    M = dz.numel() // N if N else 0
+    dx = torch.empty(dz.shape[:-1] + (K,), dtype=dz.dtype, device=dz.device) if need_dx else None
+    dw = torch.empty((N, K), dtype=dw_dtype, device=dz.device) if need_dw else None
+    if M == 0 or N == 0 or K == 0:                          # empty sums
+        return (None if dx is None else dx.zero_()), (None if dw is None else dw.zero_())
+    g = _rows(dz)
+    x2 = None if x is None else _rows(x)
+    w2 = None if weight is None else _rows(weight)
+    lib = _lib.load()
+    args = (g.data_ptr(), _pitch(g), None if x2 is None else x2.data_ptr(), 0 if x2 is None else _pitch(x2),
+            None if w2 is None else w2.data_ptr(), 0 if w2 is None else _pitch(w2))
+    with _lib.device_of(dz):
+        need = lib.act_linear_bwd_workspace(*args, M, N, K, _DTYPES[dw_dtype], need_dx, need_dw, variant)
+        ws = torch.empty(need, dtype=torch.uint8, device=dz.device) if need else None
+        rc = lib.act_linear_bwd(*args, dt, M, N, K, None if dx is None else dx.data_ptr(), K,
+                                None if dw is None else dw.data_ptr(), K, _DTYPES[dw_dtype], variant,
+                                None if ws is None else ws.data_ptr(), need, _lib.stream_ptr(dz))
+    _lib.check(rc, "act_linear_bwd")
+    return dx, dw
+
+
+def linear_status(clear: bool = True) -> int:
+    """Abort reason of the last linear_act / linear_backward kernel (0 = none).  Synchronises the device."""
+    import ctypes
+    v = ctypes.c_uint(0)
+    _lib.check(_lib.load().act_linear_status(ctypes.byref(v), 1 if clear else 0), "act_linear_status")
+    return int(v.value)

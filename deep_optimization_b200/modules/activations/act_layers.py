@@ -5,7 +5,7 @@ its eval mode compute SiLU)."""
 from torch import nn
 
 from ... import codec
-from .act_ops import _DOMaxPool2d, _DOGELU, _DOReLU, _DOSiLU
+from .act_ops import _DODropout, _DOMaxPool2d, _DOGELU, _DOReLU, _DOSiLU
 
 
 class DOReLU_Variance(nn.ReLU):
@@ -66,3 +66,22 @@ class DOMaxPool2d(nn.MaxPool2d):
                 and _square(self.dilation) == 1 and None not in (k, s, p) and codec.maxpool_supported(x, k, s, p)):
             return _DOMaxPool2d.apply(x, k, s, p)
         return super().forward(x)
+
+
+class DODropout(nn.Dropout):
+    """nn.Dropout that keeps no mask for backward: the mask comes from a counter and is made again (an
+    extension: the reference leaves dropout to PyTorch, which stores a byte per element).
+    `forward(x, residual)` returns dropout(x) + residual, in the same pass where the two share shape and
+    type.  `p` counts in 2^-16.  Follows `torch.manual_seed` and `torch.utils.checkpoint`
+    (`codec.dropout_rng`).  CPU tensors and other element types take the stock operators."""
+
+    def forward(self, x, residual=None):
+        if not (self.training and self.p > 0 and x.is_cuda and x.dtype in codec._DTYPES):
+            if residual is None:
+                return super().forward(x)
+            return nn.functional.dropout(x, self.p, self.training) + residual
+        rng = codec.dropout_rng(x.device)
+        if residual is not None and residual.shape == x.shape and residual.dtype == x.dtype and residual.device == x.device:
+            return _DODropout.apply(x, self.p, rng, residual)
+        y = _DODropout.apply(x, self.p, rng, None)
+        return y if residual is None else y + residual

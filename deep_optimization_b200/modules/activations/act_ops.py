@@ -12,6 +12,7 @@ import math
 import torch
 from torch.amp import custom_bwd, custom_fwd
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from ... import act_kernels, codec
 from ..module_utils import unified_dequantize, unified_quantize
@@ -159,3 +160,30 @@ class _DOMaxPool2d(Function):
         (idx,) = ctx.saved_tensors
         shape, k, s, pad = ctx.geom
         return codec.maxpool_bwd(idx, dy, shape, k, s, pad), None, None, None
+
+
+class _DODropout(Function):
+    """dropout(x) [+ residual] that saves the two numbers its mask is made from (`codec.dropout`)."""
+
+    @staticmethod
+    @custom_fwd(device_type="cuda")
+    def forward(ctx, input, p, rng, residual):
+        ctx.p = p
+        ctx.channels_last = codec.is_channels_last(input)      # the mask follows the input's memory order
+        if isinstance(rng, torch.Tensor):
+            ctx.rng = None
+            ctx.save_for_backward(rng)
+        else:
+            ctx.rng = rng
+        return codec.dropout(input, p, rng, residual)
+
+    @staticmethod
+    @custom_bwd(device_type="cuda")
+    @once_differentiable
+    def backward(ctx, dy):
+        rng = ctx.rng if ctx.rng is not None else ctx.saved_tensors[0]
+        dx = None
+        if ctx.needs_input_grad[0]:
+            layout = torch.channels_last if ctx.channels_last else torch.contiguous_format
+            dx = codec.dropout(dy.contiguous(memory_format=layout), ctx.p, rng)
+        return dx, None, None, dy if ctx.needs_input_grad[3] else None

@@ -4,15 +4,25 @@
 index (Model/ViT/ViT.py:39-42): three [B, heads, T, head_dim] tensors, here strided views of the
 projection's output (no copy).  Its backward hands the three gradients of the attention kernel to
 `act_merge_heads`, which writes the gradient of the projection's output directly; autograd's own
-route is a stack of the three followed by a strided copy of the result."""
+route is a stack of the three followed by a strided copy of the result.
+
+`RotaryAxes` is the split with rotary positions in it: q and k are turned by angles that grow with a
+token's coordinates on one or several axes (height and width of an image, time of a video), in the pass
+that lays the three tensors out, and their gradients are turned back in the pass that merges them.
+`rotary_split` / `rotary_merge` are its two directions without autograd."""
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
+import torch.fx
+from torch import nn
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
+from ..codec import _DTYPES
 
 
 def _merge_heads(grads, B, H, T, Dh, dtype, device):
@@ -61,3 +71,193 @@ def split_heads(qkv: torch.Tensor, heads: int):
     if qkv.is_cuda and qkv.requires_grad and qkv.is_contiguous():
         return _SplitHeads.apply(qkv, heads)
     return qkv.view(B, T, 3, heads, D3 // (3 * heads)).permute(2, 0, 3, 1, 4).unbind(0)
+
+
+# ---------------------------------------------------------------- rotary positions
+
+def rotary_turns(sections, base: float = 10000.0, device=None) -> torch.Tensor:
+    """int64 [sum(sections)]: the frequencies base ** (-i / n), i < n, of an axis with n pairs, axis after
+    axis, as 64-bit binary fractions of a turn per position.  Their products with integer positions keep
+    the fraction of the turn however far the position."""
+    if base < 1.0:
+        raise ValueError(f"rotary_turns: base must be at least 1, got {base}")
+    out = []
+    for n in sections:
+        out += [int(round(base ** (-i / n) / (2.0 * math.pi) * 2.0 ** 64)) for i in range(n)]
+    return torch.tensor(out, dtype=torch.int64, device=device)
+
+
+def _rotary_call(src, dst, rotate, positions, turns, sections, interleaved, inverse):
+    """src, dst: lists of [B, heads, T, Dh] views (last dimension contiguous), one B, T, Dh and type."""
+    ref = src[0]
+    B, _, T, Dh = ref.shape
+    if ref.dtype not in _DTYPES:
+        raise TypeError(f"unsupported activation dtype {ref.dtype}")
+    sections = tuple(int(n) for n in sections)
+    pairs = sum(sections)
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or 2 * pairs > Dh:
+        raise ValueError(f"rotary: one to four sections whose pairs fit into a head of {Dh}, got {sections}")
+    if turns.dtype != torch.int64 or turns.numel() != pairs or not turns.is_contiguous() or turns.device != ref.device:
+        raise ValueError("rotary: turns must be a contiguous int64 tensor on the tensors' device with one entry per pair")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.device != ref.device:
+        raise TypeError("rotary: positions must be int32 or int64 on the tensors' device")
+    if tuple(positions.shape) not in ((T, len(sections)), (B, T, len(sections))):
+        raise ValueError(f"rotary: positions must be [T, axes] or [B, T, axes] = [{B}, {T}, {len(sections)}], "
+                         f"got {tuple(positions.shape)}")
+    ps = positions.stride()
+    ps = ps if positions.dim() == 3 else (0,) + ps
+    n = len(src)
+    pick = lambda ts: (ctypes.c_int64 * (3 * n))(*[s for t in ts for s in (t.stride(0), t.stride(1), t.stride(2))])
+    with _lib.device_of(ref):
+        rc = _lib.load().act_rotary_heads(
+            (ctypes.c_void_p * n)(*[t.data_ptr() for t in src]), pick(src),
+            (ctypes.c_void_p * n)(*[t.data_ptr() for t in dst]), pick(dst),
+            (ctypes.c_int * n)(*[t.shape[1] for t in src]), (ctypes.c_int * n)(*rotate), n, _DTYPES[ref.dtype], B, T, Dh,
+            positions.data_ptr(), positions.element_size(), (ctypes.c_int64 * 3)(*ps), turns.data_ptr(),
+            (ctypes.c_int * len(sections))(*sections), len(sections), int(interleaved), int(inverse),
+            _lib.stream_ptr(ref))
+    _lib.check(rc, "act_rotary_heads")
+
+
+def _split_views(qkv, heads, kv_heads, Dh):
+    x = qkv.view(qkv.shape[0], qkv.shape[1], heads + 2 * kv_heads, Dh).transpose(1, 2)
+    return [x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:]]
+
+
+def rotary_split(qkv: torch.Tensor, heads: int, positions: torch.Tensor, turns: torch.Tensor, sections,
+                 kv_heads=None, interleaved: bool = False):
+    """q [B, heads, T, Dh] and k, v [B, kv_heads, T, Dh] from a fused projection's output
+    [B, T, (heads + 2 kv_heads) Dh], q and k turned; the three are views of one new buffer of qkv's
+    layout, so that qkv itself is not kept alive by them.  positions: int32 or int64 [T, axes] or
+    [B, T, axes], any values; turns: `rotary_turns(sections)`; sections: pairs per axis.  Pairs are
+    (j, P + j) in a head, or (2 j, 2 j + 1) if `interleaved`; elements behind the pairs are copied."""
+    if not qkv.is_cuda:
+        raise RuntimeError("rotary_split needs a CUDA tensor: there is no CPU path")
+    kv_heads = heads if kv_heads is None else kv_heads
+    if heads < 1 or kv_heads < 1 or qkv.dim() != 3 or qkv.shape[2] % (heads + 2 * kv_heads) or qkv.shape[2] == 0:
+        raise ValueError("rotary_split: qkv must be [B, T, (heads + 2 * kv_heads) * Dh]")
+    qkv = qkv.contiguous()
+    Dh = qkv.shape[2] // (heads + 2 * kv_heads)
+    out = torch.empty_like(qkv)
+    views = _split_views(out, heads, kv_heads, Dh)
+    _rotary_call(_split_views(qkv, heads, kv_heads, Dh), views, (1, 1, 0), positions, turns, sections, interleaved, False)
+    return tuple(views)
+
+
+def rotary_merge(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor,
+                 sections, interleaved: bool = False) -> torch.Tensor:
+    """The gradient of `rotary_split`'s qkv from the gradients of its q, k and v (any strides): dq and dk
+    turned back, the three merged, one pass."""
+    if not dq.is_cuda:
+        raise RuntimeError("rotary_merge needs CUDA tensors: there is no CPU path")
+    B, H, T, Dh = dq.shape
+    K = dk.shape[1]
+    if dk.shape != (B, K, T, Dh) or dv.shape != dk.shape or len({dq.dtype, dk.dtype, dv.dtype}) != 1 \
+            or len({dq.device, dk.device, dv.device}) != 1:
+        raise ValueError("rotary_merge: dq [B, heads, T, Dh] and dk, dv [B, kv_heads, T, Dh] of one type and device")
+    grads = [g if g.stride(3) == 1 or Dh == 1 else g.contiguous() for g in (dq, dk, dv)]
+    out = torch.empty((B, T, (H + 2 * K) * Dh), dtype=dq.dtype, device=dq.device)
+    _rotary_call(grads, _split_views(out, H, K, Dh), (1, 1, 0), positions, turns, sections, interleaved, True)
+    return out
+
+
+def rotary_heads(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, sections, interleaved: bool = False,
+                 inverse: bool = False) -> torch.Tensor:
+    """One [B, heads, T, Dh] tensor (any strides) turned, or turned back; the result is contiguous."""
+    if not x.is_cuda:
+        raise RuntimeError("rotary_heads needs a CUDA tensor: there is no CPU path")
+    if x.dim() != 4:
+        raise ValueError("rotary_heads: x must be [B, heads, T, Dh]")
+    if x.stride(3) != 1:
+        x = x.contiguous()
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _rotary_call([x], [out], (1,), positions, turns, sections, interleaved, inverse)
+    return out
+
+
+class _RotarySplit(Function):
+    @staticmethod
+    def forward(ctx, qkv, heads, positions, turns, sections, kv_heads, interleaved):
+        ctx.save_for_backward(positions, turns)
+        ctx.how = (sections, interleaved)
+        ctx.set_materialize_grads(False)
+        q, k, v = rotary_split(qkv, heads, positions, turns, sections, kv_heads, interleaved)
+        ctx.like = (q.shape, k.shape)
+        return q, k, v
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk, dv):
+        positions, turns = ctx.saved_tensors
+        sections, interleaved = ctx.how
+        ref = next((g for g in (dq, dk, dv) if g is not None), None)
+        if ref is None:
+            return (None,) * 7
+        grads = [torch.zeros(s, dtype=ref.dtype, device=ref.device) if g is None else g.to(ref.dtype)
+                 for g, s in ((dq, ctx.like[0]), (dk, ctx.like[1]), (dv, ctx.like[1]))]
+        return rotary_merge(*grads, positions, turns, sections, interleaved), None, None, None, None, None, None
+
+
+class _RotaryHeads(Function):
+    @staticmethod
+    def forward(ctx, x, positions, turns, sections, interleaved):
+        ctx.save_for_backward(positions, turns)
+        ctx.how = (sections, interleaved)
+        return rotary_heads(x, positions, turns, sections, interleaved)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        positions, turns = ctx.saved_tensors
+        sections, interleaved = ctx.how
+        return rotary_heads(dy, positions, turns, sections, interleaved, inverse=True), None, None, None, None
+
+
+def rotary_split_heads(qkv, heads, positions, turns, sections, kv_heads=None, interleaved=False):
+    """`rotary_split` that differentiates (once) with respect to qkv.  Tensors on the meta device get the
+    results' shapes, which is what shape propagation asks for."""
+    if qkv.is_meta:
+        K = heads if kv_heads is None else kv_heads
+        return tuple(_split_views(qkv, heads, K, qkv.shape[2] // (heads + 2 * K)))
+    return _RotarySplit.apply(qkv, heads, positions, turns, sections, kv_heads, interleaved)
+
+
+def rotary_turn_heads(x, positions, turns, sections, interleaved=False):
+    """`rotary_heads` that differentiates (once) with respect to x."""
+    if x.is_meta:
+        return torch.empty_like(x)
+    return _RotaryHeads.apply(x, positions, turns, sections, interleaved)
+
+
+# leaves for torch.fx: a trace keeps the calls that RotaryAxes makes, not their branches
+torch.fx.wrap("rotary_split_heads")
+torch.fx.wrap("rotary_turn_heads")
+
+
+class RotaryAxes(nn.Module):
+    """Rotary positions with one to four axes.  `sections` are the pairs of a head that each axis turns
+    (their sum at most half the head); `base` sets the frequencies base ** (-i / n).
+
+    `forward(qkv, heads, positions, kv_heads=None)` splits a fused projection's output as `split_heads`
+    does, q and k turned; `turn(x, positions)` turns one [B, heads, T, Dh] tensor.  Both differentiate
+    (once) with respect to their tensor.  positions: integers, [T, axes] or [B, T, axes]; a token at the
+    origin, such as a class token, is not turned."""
+
+    def __init__(self, sections, base: float = 10000.0, interleaved: bool = False):
+        super().__init__()
+        self.sections, self.base, self.interleaved = tuple(int(n) for n in sections), float(base), bool(interleaved)
+        self.register_buffer("turns", rotary_turns(self.sections, self.base), persistent=False)
+
+    def forward(self, qkv, heads, positions, kv_heads=None):
+        return rotary_split_heads(qkv, heads, positions, self.turns, self.sections, kv_heads, self.interleaved)
+
+    def turn(self, x, positions):
+        return rotary_turn_heads(x, positions, self.turns, self.sections, self.interleaved)
+
+
+def image_positions(height: int, width: int, leading: int = 1, device=None) -> torch.Tensor:
+    """int64 [leading + height * width, 2]: the row and column, counted from 1, of the patches of an image
+    in row-major order, behind `leading` tokens at the origin (a class token)."""
+    y, x = torch.meshgrid(torch.arange(1, height + 1), torch.arange(1, width + 1), indexing="ij")
+    grid = torch.stack([y.reshape(-1), x.reshape(-1)], -1)
+    return torch.cat([torch.zeros(leading, 2, dtype=torch.int64), grid]).to(device)

@@ -42,9 +42,17 @@ extern "C" {
 #define ACT_FLAG_BALLOT_REF_BIAS 32 /* act_pack_ballot: keep the reference's extra -0.5 in the rounding */
 
 /* activation kinds of act_activation_fwd_quant_pack */
+#define ACT_KIND_NONE 0            /* act_linear_fwd only, as is ACT_KIND_RELU */
 #define ACT_KIND_GELU 1            /* tanh-approximated GELU */
 #define ACT_KIND_SILU 2
 #define ACT_KIND_GELU_ERF 3        /* exact GELU, x * Phi(x) */
+#define ACT_KIND_RELU 4
+
+/* kernel choice of act_linear_fwd / act_linear_bwd: 0 leaves it to the library */
+#define ACT_LINEAR_PAIR 1          /* CTA pairs on 256 x 256 tiles */
+#define ACT_LINEAR_128 2           /* one CTA per 128 x 128 tile */
+#define ACT_LINEAR_64 3            /* one CTA per 128 x 64 tile */
+#define ACT_LINEAR_FEW_ROWS 4      /* forward, up to eight rows: a warp per column, no tensor cores */
 
 /* flags of act_fp8_gemm */
 #define ACT_GEMM_B_IS_NK 1         /* B is stored [N,K] (K contiguous, like nn.Linear weights)        */
@@ -434,6 +442,77 @@ ACT_API int act_ln_bwd_from_packed_sum(const void* dy, const void* dy2, int dtyp
  */
 ACT_API int act_merge_heads(const void* const* srcs, const int64_t* strides, int parts, int B, int H, int T,
                             int Dh, int elem_bytes, void* dst, void* stream);
+
+/*
+ * Linear layer with bias, activation and residual in the product's epilogue, bf16 or fp16 (dtype, all
+ * operands and outputs but where said), fp32 sums:
+ *   act_linear_fwd:  y[m, n] = f(z) + residual[m, n], z = sum_k x[m, k] w[n, k] + bias[n], rounded once;
+ *       deriv (may be NULL; GELU and SiLU kinds only) receives f'(z), what a layer that saves the
+ *       activation's derivative compressed needs for its backward pass.  kind: ACT_KIND_*.  bias (may
+ *       be NULL) is bf16, fp16 or fp32.  residual may be NULL and may be y.
+ *   act_mul_col_sum: dz = dy * d (rounded once) and db[n] = sum_m dy * d before that rounding (fp32,
+ *       may be NULL), contiguous [M, N]; the gradient of z and of the bias in one pass.
+ *   act_linear_bwd:  dx = dz w and dw = dz^T x (either may be NULL); dw in dtype or fp32.
+ * ld_* are row pitches in elements, any alignment: operands whose rows are not 16-byte aligned are
+ * copied into the workspace first, outputs like that are written element by element.  The
+ * *_workspace functions say how many bytes (16-byte aligned) a call with these arguments takes, 0
+ * included.  Sums that are split over CTAs are joined in a fixed order: results are repeatable.
+ * Replaces F.linear followed by the activation and the addition, and the two products of
+ * _DOLinear.backward (AC/modules/ops.py:438-540).
+ */
+ACT_API size_t act_linear_fwd_workspace(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int M, int N, int K, int variant);
+ACT_API int act_linear_fwd(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* bias, int bias_dtype,
+                           const void* residual, int64_t ld_r, int dtype, int M, int N, int K, int kind,
+                           void* y, int64_t ld_y, void* deriv, int64_t ld_d, int variant,
+                           void* workspace, size_t ws_bytes, void* stream);
+ACT_API size_t act_mul_col_sum_workspace(int64_t M, int N);
+ACT_API int act_mul_col_sum(const void* dy, const void* d, int dtype, int64_t M, int N, void* dz, float* db,
+                            void* workspace, size_t ws_bytes, void* stream);
+ACT_API size_t act_linear_bwd_workspace(const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, const void* w, int64_t ld_w,
+                                        int M, int N, int K, int dw_dtype, int need_dx, int need_dw, int variant);
+ACT_API int act_linear_bwd(const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, const void* w, int64_t ld_w, int dtype,
+                           int M, int N, int K, void* dx, int64_t ld_dx, void* dw, int64_t ld_dw, int dw_dtype, int variant,
+                           void* workspace, size_t ws_bytes, void* stream);
+/* Abort reason of the last tensor-core kernel of these on the current device (0 = none); synchronises. */
+ACT_API int act_linear_status(unsigned int* out, int clear);
+
+/*
+ * Dropout whose mask is a function of (seed, offset, element index) and never stored:
+ *     y[e] = (h(e) >= threshold ? x[e] * 65536 / (65536 - threshold) : 0) + residual[e]
+ * h(e): the (e & 7)th sixteen bits, low half of a word first, of the Philox-4x32-10 block with
+ * counter (e >> 3, offset) and key seed.  The backward pass is the same call on dy without the
+ * residual.  No counterpart in the reference (its payloads leave dropout to PyTorch).
+ *   x, residual (may be NULL), y: n elements of dtype, aligned to the element; y may be x or residual
+ *   threshold: the dropping probability in 2^-16, 0..65536 (65536 drops everything)
+ *   rng: NULL, or two 64-bit words on the device, seed and offset, that replace the arguments
+ *        (8-byte aligned; what act_rng_ticket writes), for launches inside a captured graph
+ * act_rng_ticket: out = {state[0], state[1]}, then state[1] += 1, atomically; state and out are two
+ * 64-bit words each on the device.
+ */
+ACT_API int act_dropout(const void* x, const void* residual, int dtype, int64_t n, unsigned threshold, uint64_t seed,
+                        uint64_t offset, const void* rng, void* y, void* stream);
+ACT_API int act_rng_ticket(void* state, void* out, void* stream);
+
+/*
+ * Rotary positions with up to four axes on up to three [B, heads, T, Dh] tensors of one B and T in
+ * one pass (q, k, v; heads may differ per tensor, a tensor with rotate[s] = 0 is copied).  Pair j of
+ * a head is turned by pos[b, t, axis(j)] * turns[j]; pairs are (j, P + j), or (2 j, 2 j + 1) with
+ * `interleaved`, P = the sum of sections; elements from 2 P on are copied.  `inverse` negates the
+ * angles (the backward pass).  Stands next to act_merge_heads: the q/k/v split of a fused projection
+ * and its backward with the rotation in them (the reference has learned positions only,
+ * Model/ViT/ViT.py:111).
+ *   srcs, dsts: parts pointers each, aligned to the element; dst may be src with the same strides,
+ *       but must not overlap it otherwise; *_strides: element strides (batch, head, token) per part,
+ *       the last dimension contiguous
+ *   pos: int32 or int64 (pos_bytes 4 or 8), element strides (batch, token, axis), any values
+ *   turns: P frequencies as 64-bit binary fractions of a turn per position, round(2^64 f / 2 pi)
+ *   sections (host): pairs of each axis, in the order of turns
+ */
+ACT_API int act_rotary_heads(const void* const* srcs, const int64_t* src_strides, void* const* dsts,
+                             const int64_t* dst_strides, const int* heads, const int* rotate, int parts, int dtype,
+                             int64_t B, int64_t T, int Dh, const void* pos, int pos_bytes, const int64_t* pos_strides,
+                             const void* turns, const int* sections, int axes, int interleaved, int inverse,
+                             void* stream);
 
 /*
  * Greedy bit allocation on the host (no GPU work).
