@@ -90,6 +90,10 @@ SIGNATURES = {
     "act_rng_ticket": ([_vp, _vp, _vp], _i32),
     "act_rotary_heads": ([_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i64, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _i32, _i32,
                           _i32, _vp], _i32),
+    "act_rotary_split": ([_vp, _vp, _i32, _i32, _i32, _i64, _i64, _i32, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _i32, _vp],
+                         _i32),
+    "act_rotary_merge": ([_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _i64, _i32, _vp, _i32, _i64, _i64, _i64, _vp, _vp,
+                          _i32, _i32, _vp], _i32),
     "act_calc_precision": ([_vp, _vp, _vp, _i64, ctypes.c_double], _i32),
     "act_fp8_gemm_workspace": ([_i32, _i32, _i32, _i32], ctypes.c_size_t),
     "act_fp8_gemm": ([_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, ctypes.c_size_t, _vp], _i32),

@@ -174,7 +174,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     lib = _lib.load()
     xp, wp, ldx, ldw = x2.data_ptr(), w2.data_ptr(), _pitch(x2), _pitch(w2)
     ws_ptr = ws = None
-    need = lib.act_linear_fwd_workspace(xp, ldx, wp, ldw, M, N, K, variant)
+    need = 0
+    if (xp | wp) & 15 or (ldx | ldw) & 7:                  # rows that may have to be copied first
+        need = lib.act_linear_fwd_workspace(xp, ldx, wp, ldw, M, N, K, variant)
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
         ws_ptr = ws.data_ptr()

@@ -13,6 +13,7 @@ that lays the three tensors out, and their gradients are turned back in the pass
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -87,41 +88,50 @@ def rotary_turns(sections, base: float = 10000.0, device=None) -> torch.Tensor:
     return torch.tensor(out, dtype=torch.int64, device=device)
 
 
-def _rotary_call(src, dst, rotate, positions, turns, sections, interleaved, inverse):
-    """src, dst: lists of [B, heads, T, Dh] views (last dimension contiguous), one B, T, Dh and type."""
-    ref = src[0]
-    B, _, T, Dh = ref.shape
-    if ref.dtype not in _DTYPES:
-        raise TypeError(f"unsupported activation dtype {ref.dtype}")
-    sections = tuple(int(n) for n in sections)
-    pairs = sum(sections)
-    if not 1 <= len(sections) <= 4 or min(sections) < 0 or 2 * pairs > Dh:
-        raise ValueError(f"rotary: one to four sections whose pairs fit into a head of {Dh}, got {sections}")
-    if turns.dtype != torch.int64 or turns.numel() != pairs or not turns.is_contiguous() or turns.device != ref.device:
+_I64x3, _I64x9 = ctypes.c_int64 * 3, ctypes.c_int64 * 9
+
+
+@functools.lru_cache(maxsize=64)
+def _sections_array(sections):
+    """The C array of a tuple of pair counts, and their sum."""
+    if not 1 <= len(sections) <= 4 or min(sections) < 0:
+        raise ValueError(f"rotary: one to four sections of zero or more pairs, got {sections}")
+    return (ctypes.c_int * len(sections))(*sections), sum(sections)
+
+
+def _rotary_args(ref, B, T, Dh, positions, turns, sections):
+    """Checks, and (pos pointer, bytes, three strides, turns pointer, sections, axes) for the library."""
+    array, pairs = _sections_array(tuple(sections))
+    axes = len(array)
+    if 2 * pairs > Dh:
+        raise ValueError(f"rotary: the sections' pairs {tuple(sections)} do not fit into a head of {Dh}")
+    dev = ref.device
+    if turns.dtype != torch.int64 or turns.numel() != pairs or turns.device != dev or not turns.is_contiguous():
         raise ValueError("rotary: turns must be a contiguous int64 tensor on the tensors' device with one entry per pair")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.device != ref.device:
+    es = 8 if positions.dtype == torch.int64 else 4
+    if (es == 4 and positions.dtype != torch.int32) or positions.device != dev:
         raise TypeError("rotary: positions must be int32 or int64 on the tensors' device")
-    if tuple(positions.shape) not in ((T, len(sections)), (B, T, len(sections))):
-        raise ValueError(f"rotary: positions must be [T, axes] or [B, T, axes] = [{B}, {T}, {len(sections)}], "
-                         f"got {tuple(positions.shape)}")
-    ps = positions.stride()
-    ps = ps if positions.dim() == 3 else (0,) + ps
-    n = len(src)
-    pick = lambda ts: (ctypes.c_int64 * (3 * n))(*[s for t in ts for s in (t.stride(0), t.stride(1), t.stride(2))])
-    with _lib.device_of(ref):
-        rc = _lib.load().act_rotary_heads(
-            (ctypes.c_void_p * n)(*[t.data_ptr() for t in src]), pick(src),
-            (ctypes.c_void_p * n)(*[t.data_ptr() for t in dst]), pick(dst),
-            (ctypes.c_int * n)(*[t.shape[1] for t in src]), (ctypes.c_int * n)(*rotate), n, _DTYPES[ref.dtype], B, T, Dh,
-            positions.data_ptr(), positions.element_size(), (ctypes.c_int64 * 3)(*ps), turns.data_ptr(),
-            (ctypes.c_int * len(sections))(*sections), len(sections), int(interleaved), int(inverse),
-            _lib.stream_ptr(ref))
-    _lib.check(rc, "act_rotary_heads")
+    shape = positions.shape
+    if shape == (T, axes):
+        st, sa = positions.stride()
+        sb = 0
+    elif shape == (B, T, axes):
+        sb, st, sa = positions.stride()
+    else:
+        raise ValueError(f"rotary: positions must be [T, axes] or [B, T, axes] = [{B}, {T}, {axes}], got {tuple(shape)}")
+    return positions.data_ptr(), es, sb, st, sa, turns.data_ptr(), array, axes
 
 
 def _split_views(qkv, heads, kv_heads, Dh):
     x = qkv.view(qkv.shape[0], qkv.shape[1], heads + 2 * kv_heads, Dh).transpose(1, 2)
-    return [x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:]]
+    return x.split((heads, kv_heads, kv_heads), 1)
+
+
+def _dtype_code(t):
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"unsupported activation dtype {t.dtype}")
+    return code
 
 
 def rotary_split(qkv: torch.Tensor, heads: int, positions: torch.Tensor, turns: torch.Tensor, sections,
@@ -137,11 +147,15 @@ def rotary_split(qkv: torch.Tensor, heads: int, positions: torch.Tensor, turns: 
     if heads < 1 or kv_heads < 1 or qkv.dim() != 3 or qkv.shape[2] % (heads + 2 * kv_heads) or qkv.shape[2] == 0:
         raise ValueError("rotary_split: qkv must be [B, T, (heads + 2 * kv_heads) * Dh]")
     qkv = qkv.contiguous()
-    Dh = qkv.shape[2] // (heads + 2 * kv_heads)
+    B, T, W = qkv.shape
+    Dh = W // (heads + 2 * kv_heads)
+    pos, es, sb, st, sa, tp, array, axes = _rotary_args(qkv, B, T, Dh, positions, turns, sections)
     out = torch.empty_like(qkv)
-    views = _split_views(out, heads, kv_heads, Dh)
-    _rotary_call(_split_views(qkv, heads, kv_heads, Dh), views, (1, 1, 0), positions, turns, sections, interleaved, False)
-    return tuple(views)
+    with _lib.device_of(qkv):
+        rc = _lib.load().act_rotary_split(qkv.data_ptr(), out.data_ptr(), heads, kv_heads, _dtype_code(qkv), B, T, Dh, pos, es,
+                                          sb, st, sa, tp, array, axes, int(interleaved), _lib.stream_ptr(qkv))
+    _lib.check(rc, "act_rotary_split")
+    return tuple(_split_views(out, heads, kv_heads, Dh))
 
 
 def rotary_merge(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor,
@@ -152,12 +166,21 @@ def rotary_merge(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, positions
         raise RuntimeError("rotary_merge needs CUDA tensors: there is no CPU path")
     B, H, T, Dh = dq.shape
     K = dk.shape[1]
-    if dk.shape != (B, K, T, Dh) or dv.shape != dk.shape or len({dq.dtype, dk.dtype, dv.dtype}) != 1 \
-            or len({dq.device, dk.device, dv.device}) != 1:
+    if dk.shape != (B, K, T, Dh) or dv.shape != dk.shape or dk.dtype != dq.dtype or dv.dtype != dq.dtype \
+            or dk.device != dq.device or dv.device != dq.device:
         raise ValueError("rotary_merge: dq [B, heads, T, Dh] and dk, dv [B, kv_heads, T, Dh] of one type and device")
-    grads = [g if g.stride(3) == 1 or Dh == 1 else g.contiguous() for g in (dq, dk, dv)]
+    pos, es, sb, st, sa, tp, array, axes = _rotary_args(dq, B, T, Dh, positions, turns, sections)
+    (q0, q1, q2, q3), (k0, k1, k2, k3), (v0, v1, v2, v3) = dq.stride(), dk.stride(), dv.stride()
+    if not q3 == k3 == v3 == 1:
+        dq, dk, dv = dq.contiguous(), dk.contiguous(), dv.contiguous()
+        (q0, q1, q2, _), (k0, k1, k2, _), (v0, v1, v2, _) = dq.stride(), dk.stride(), dv.stride()
     out = torch.empty((B, T, (H + 2 * K) * Dh), dtype=dq.dtype, device=dq.device)
-    _rotary_call(grads, _split_views(out, H, K, Dh), (1, 1, 0), positions, turns, sections, interleaved, True)
+    with _lib.device_of(dq):
+        rc = _lib.load().act_rotary_merge(dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                          _I64x9(q0, q1, q2, k0, k1, k2, v0, v1, v2), out.data_ptr(), H, K, _dtype_code(dq),
+                                          B, T, Dh, pos, es, sb, st, sa, tp, array, axes, int(interleaved),
+                                          _lib.stream_ptr(dq))
+    _lib.check(rc, "act_rotary_merge")
     return out
 
 
@@ -170,8 +193,18 @@ def rotary_heads(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, 
         raise ValueError("rotary_heads: x must be [B, heads, T, Dh]")
     if x.stride(3) != 1:
         x = x.contiguous()
+    B, H, T, Dh = x.shape
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _rotary_call([x], [out], (1,), positions, turns, sections, interleaved, inverse)
+    if x.numel() == 0:
+        return out
+    pos, es, sb, st, sa, tp, array, axes = _rotary_args(x, B, T, Dh, positions, turns, sections)
+    one = ctypes.c_int * 1
+    with _lib.device_of(x):
+        rc = _lib.load().act_rotary_heads(
+            (ctypes.c_void_p * 1)(x.data_ptr()), _I64x3(*x.stride()[:3]), (ctypes.c_void_p * 1)(out.data_ptr()),
+            _I64x3(*out.stride()[:3]), one(H), one(1), 1, _dtype_code(x), B, T, Dh, pos, es, _I64x3(sb, st, sa), tp, array,
+            axes, int(interleaved), int(inverse), _lib.stream_ptr(x))
+    _lib.check(rc, "act_rotary_heads")
     return out
 
 

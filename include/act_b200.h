@@ -513,6 +513,16 @@ ACT_API int act_rotary_heads(const void* const* srcs, const int64_t* src_strides
                              int64_t B, int64_t T, int Dh, const void* pos, int pos_bytes, const int64_t* pos_strides,
                              const void* turns, const int* sections, int axes, int interleaved, int inverse,
                              void* stream);
+/* The two common uses: a contiguous [B, T, (heads + 2 kv_heads) Dh] projection output into dst of the same
+ * layout, q and k turned; and the gradients dq, dk, dv (src_strides: 3 x (batch, head, token)) turned back
+ * and merged into the gradient of that output. */
+ACT_API int act_rotary_split(const void* qkv, void* dst, int heads, int kv_heads, int dtype, int64_t B, int64_t T, int Dh,
+                             const void* pos, int pos_bytes, int64_t pos_sb, int64_t pos_st, int64_t pos_sa,
+                             const void* turns, const int* sections, int axes, int interleaved, void* stream);
+ACT_API int act_rotary_merge(const void* dq, const void* dk, const void* dv, const int64_t* src_strides, void* dst,
+                             int heads, int kv_heads, int dtype, int64_t B, int64_t T, int Dh, const void* pos,
+                             int pos_bytes, int64_t pos_sb, int64_t pos_st, int64_t pos_sa, const void* turns,
+                             const int* sections, int axes, int interleaved, void* stream);
 
 /*
  * Greedy bit allocation on the host (no GPU work).

@@ -129,6 +129,18 @@ def test_rotary_refusals(lib):
     assert _rotary(lib, B=0) == 0 and _rotary(lib, T=0) == 0 and _rotary(lib, heads=0) == 0
 
 
+def test_rotary_split_and_merge_refusals(lib):
+    sec = (ctypes.c_int * 1)(16)
+    split = lambda q=P, o=P, h=2, k=1, dt=1, T=4, Dh=64: lib.act_rotary_split(q, o, h, k, dt, 1, T, Dh, P, 8, 0, 1, 1, P, sec, 1, 0, None)
+    assert split(dt=4) == DTYPE and split(h=-1) == SIZE and split(T=-1) == SIZE and split(Dh=0) == SIZE and split(Dh=31) == SIZE
+    assert split(q=None) == NULL and split(o=None) == NULL and split(q=ODD) == ALIGN and split(T=0) == 0
+    st = (ctypes.c_int64 * 9)(*([256, 64, 64] * 3))
+    merge = lambda q=P, k=P, v=P, o=P, dt=1, T=4, Dh=64: lib.act_rotary_merge(q, k, v, st, o, 2, 1, dt, 1, T, Dh, P, 8, 0, 1, 1, P, sec, 1, 0, None)
+    assert merge(dt=4) == DTYPE and merge(T=-1) == SIZE and merge(Dh=31) == SIZE
+    assert merge(q=None) == NULL and merge(k=None) == NULL and merge(v=None) == NULL and merge(o=None) == NULL
+    assert merge(v=ODD) == ALIGN and merge(T=0) == 0
+
+
 def test_cpu_tensors_are_refused():
     from deep_optimization_b200 import gemm
     from deep_optimization_b200.modules import attention
