@@ -86,10 +86,10 @@ __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
 __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
 __device__ __forceinline__ uint32_t cluster_ctarank() {
@@ -112,6 +112,23 @@ template <int CG> __device__ __forceinline__ void sync_all() {
 __device__ __forceinline__ void fence_barrier_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // operand load; the bytes are counted on the leader's barrier (`bar`: its cluster address)
+// (`dst`: its shared-memory address; `on`: whether this thread issues it)
+template <int CG> __device__ __forceinline__ void tma_load_if(uint32_t on, uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    if (CG == 2)
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+                     "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+                     :: "r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(on) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+                     "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+                     :: "r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(on) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx_if(uint32_t on, uint32_t bar, uint32_t bytes) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}"
+                 :: "r"(bar), "r"(bytes), "r"(on) : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" :: "l"(map) : "memory"); }
+// residual load, one CTA's own
 template <int CG> __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
     if (CG == 2)
         asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -146,22 +163,23 @@ template <int CG> __device__ __forceinline__ void tmem_dealloc(uint32_t taddr) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-template <int CG> __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+template <int CG> __device__ __forceinline__ void umma_if(uint32_t on, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     if (CG == 2)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                     :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                     :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
 }
 // arrives, once the MMAs issued so far are done, on the barrier at this offset (in both CTAs of a pair)
-template <int CG> __device__ __forceinline__ void umma_commit(uint64_t* bar) {
+template <int CG> __device__ __forceinline__ void umma_commit_if(uint32_t on, uint32_t bar) {
     if (CG == 2) {
         const uint16_t both = 3;
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                     :: "r"(smem_u32(bar)), "h"(both) : "memory");
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+                     :: "r"(bar), "h"(both), "r"(on) : "memory");
     } else {
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                     :: "r"(bar), "r"(on) : "memory");
     }
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
@@ -176,17 +194,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// A wait that runs out records why and raises this CTA's abort flag and its peer's.
+// A wait that runs out records why and raises this CTA's abort flag and its peer's.  Every lane of the
+// warp waits, so that the loops around it stay uniform over the warp.
 template <int CG, typename S>
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, S* s, uint32_t code, uint32_t peer_abort) {
-    for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (s->abort) return false;
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, S* s, uint32_t code, uint32_t peer_abort) {
+    bool ok = mbar_try_wait(bar, parity);
+    for (uint32_t i = 0; !ok && i < SPIN_LIMIT && !s->abort; ++i) ok = mbar_try_wait(bar, parity);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok && !s->abort && (threadIdx.x & 31) == 0) {
+        s->abort = 1;
+        if (CG == 2) st_cluster_u32(peer_abort, 1u);
+        atomicExch(&g_linear_error, code);
     }
-    s->abort = 1;
-    if (CG == 2) st_cluster_u32(peer_abort, 1u);
-    atomicExch(&g_linear_error, code);
-    return false;
+    return ok;
 }
 // warp-wide: lane 0 polls with a short sleep in between, everybody learns the outcome
 template <int CG, typename S>
@@ -195,7 +215,7 @@ __device__ __forceinline__ bool wait_bar_warp(uint64_t* bar, uint32_t parity, S*
     if ((threadIdx.x & 31) == 0) {
         ok = 0;
         for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
-            if (mbar_try_wait(bar, parity)) { ok = 1; break; }
+            if (mbar_try_wait(smem_u32(bar), parity)) { ok = 1; break; }
             if (s->abort) break;
             __nanosleep(32);
         }
@@ -207,8 +227,8 @@ __device__ __forceinline__ bool wait_bar_warp(uint64_t* bar, uint32_t parity, S*
 // Shared-memory descriptor of an operand tile with the 128-byte swizzle.  K-major: rows of the M or N
 // index, eight-row groups 1024 bytes apart, the leading offset unused.  MN-major: rows of the
 // reduction index, eight-row groups 1024 bytes apart, chunks of 64 columns CHUNK bytes apart.
-__device__ __forceinline__ uint64_t make_desc(const void* tile, bool mn_major) {
-    uint64_t d = (uint64_t)((smem_u32(tile) & 0x3FFFF) >> 4);
+__device__ __forceinline__ uint64_t make_desc(uint32_t tile, bool mn_major) {
+    uint64_t d = (uint64_t)((tile & 0x3FFFF) >> 4);
     d |= (mn_major ? (uint64_t)(CHUNK >> 4) : (uint64_t)1) << 16;
     d |= (uint64_t)(1024 >> 4) << 32;
     d |= (uint64_t)1 << 46;                          // descriptor version
@@ -309,7 +329,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     using S = Smem<CG, BN>;
     extern __shared__ __align__(1024) uint8_t smem_raw_linear[];
     S* s = reinterpret_cast<S*>(smem_raw_linear);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform, and known to be
     const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;      // 0 = leader
     const int m_tiles = (p.M + C::TILE_M - 1) / C::TILE_M, n_tiles = (p.N + BN - 1) / BN;
     const int n_work = m_tiles * n_tiles * p.slices;
@@ -328,6 +348,11 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         s->abort = 0;
         fence_barrier_init();
     }
+    if (warp == 0 && lane == 0) {
+        prefetch_map(&map_a);
+        prefetch_map(&map_b);
+        if (p.out_f32 || p.tma_out) prefetch_map(&map_y);
+    }
     if (warp == 1) tmem_alloc<CG>(&s->tmem_base);                 // the same warp of both CTAs
     tc_fence_before();
     sync_all<CG>();                                               // barriers of both CTAs exist from here on
@@ -341,46 +366,52 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         hi = lo + per + (sl < extra ? 1 : 0);
     };
 
+    // The producer's and the issuer's loops run on a whole warp, uniform over it, and one lane's
+    // predicate guards each load, MMA and commit: the operands then sit in uniform registers, where
+    // these instructions take them from.  As the loop of a single lane the issuer needed about 600
+    // cycles per 64 of the reduction, whatever the tile ([16, 4096] x [4096, 4096]: 25 us).
+    const uint32_t one = lane == 0;
+    const uint32_t full0 = smem_u32(&s->full[0]), empty0 = smem_u32(&s->empty[0]);
+    const uint32_t a0 = smem_u32(&s->a[0][0]), b0 = smem_u32(&s->b[0][0]);
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer
-        if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
-            bool ok = true;
-            for (int w = first; ok && w < n_work; w += stride) {
-                const int tile = w / p.slices, m0 = (tile / n_tiles) * C::TILE_M + (int)rank * BM;
-                const int n0 = (tile % n_tiles) * BN + (int)rank * C::BNC;
-                int lo, hi;
-                slice_range(w % p.slices, lo, hi);
-                for (int kb = lo; kb < hi; ++kb) {
-                    if (!(ok = wait_bar<CG>(&s->empty[stage], phase ^ 1, s, 1, peer_abort))) break;
-                    // the leader's barrier counts the bytes of both CTAs; parts out of range arrive as zeros
-                    if (rank == 0) mbar_expect_tx(&s->full[stage], CG * (C::A_STAGE + C::B_STAGE));
-                    const uint32_t bar = CG == 2 ? map_to_cta(smem_u32(&s->full[stage]), 0) : smem_u32(&s->full[stage]);
-                    if (p.a_mn) {
+        uint32_t stage = 0, phase = 0;
+        bool ok = true;
+        const uint32_t lead_full0 = CG == 2 ? map_to_cta(full0, 0) : full0;
+        for (int w = first; ok && w < n_work; w += stride) {
+            const int tile = w / p.slices, m0 = (tile / n_tiles) * C::TILE_M + (int)rank * BM;
+            const int n0 = (tile % n_tiles) * BN + (int)rank * C::BNC;
+            int lo, hi;
+            slice_range(w % p.slices, lo, hi);
+            for (int kb = lo; kb < hi; ++kb) {
+                if (!(ok = wait_bar<CG>(empty0 + 8 * stage, phase ^ 1, s, 1, peer_abort))) break;
+                // the leader's barrier counts the bytes of both CTAs; parts out of range arrive as zeros
+                if (rank == 0) mbar_expect_tx_if(one, full0 + 8 * stage, CG * (C::A_STAGE + C::B_STAGE));
+                const uint32_t bar = lead_full0 + 8 * stage, at = a0 + stage * C::A_STAGE, bt = b0 + stage * C::B_STAGE;
+                if (p.a_mn) {
 #pragma unroll
-                        for (int c = 0; c < BM / 64; ++c) tma_load<CG>(s->a[stage] + c * CHUNK, &map_a, bar, m0 + c * 64, kb * BK);
-                    } else {
-                        tma_load<CG>(s->a[stage], &map_a, bar, kb * BK, m0);
-                    }
-                    if (p.b_mn) {
-#pragma unroll
-                        for (int c = 0; c < C::BNC / 64; ++c) tma_load<CG>(s->b[stage] + c * CHUNK, &map_b, bar, n0 + c * 64, kb * BK);
-                    } else {
-                        tma_load<CG>(s->b[stage], &map_b, bar, kb * BK, n0);
-                    }
-                    if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
+                    for (int c = 0; c < BM / 64; ++c) tma_load_if<CG>(one, at + c * CHUNK, &map_a, bar, m0 + c * 64, kb * BK);
+                } else {
+                    tma_load_if<CG>(one, at, &map_a, bar, kb * BK, m0);
                 }
-            }
-            // every slot handed out has come back: no arrival of the leader's commits is still on its
-            // way to this CTA's barriers when it leaves
-            for (int i = 0; ok && i < C::STAGES; ++i) {
-                ok = wait_bar<CG>(&s->empty[stage], phase ^ 1, s, 6, peer_abort);
+                if (p.b_mn) {
+#pragma unroll
+                    for (int c = 0; c < C::BNC / 64; ++c) tma_load_if<CG>(one, bt + c * CHUNK, &map_b, bar, n0 + c * 64, kb * BK);
+                } else {
+                    tma_load_if<CG>(one, bt, &map_b, bar, kb * BK, n0);
+                }
                 if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
             }
         }
+        // every slot handed out has come back: no arrival of the leader's commits is still on its
+        // way to this CTA's barriers when it leaves
+        for (int i = 0; ok && i < C::STAGES; ++i) {
+            ok = wait_bar<CG>(empty0 + 8 * stage, phase ^ 1, s, 6, peer_abort);
+            if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
+        }
     } else if (warp == 1) {
         // -------------------------------------------------------------- MMA issuer (the leader's)
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             // fp32 accumulate; A and B f16 (0) or bf16 (1); operand majors; N / 8; M / 16
             const uint32_t t16 = p.dtype == ACT_DTYPE_BF16 ? 1u : 0u;
             const uint32_t idesc = (1u << 4) | (t16 << 7) | (t16 << 10) | ((uint32_t)(p.a_mn != 0) << 15) | ((uint32_t)(p.b_mn != 0) << 16) |
@@ -388,30 +419,30 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             // K = 16 further on: 32 bytes of a K-major row, or 16 rows of 128 bytes
             const uint64_t a_step = p.a_mn ? (uint64_t)((UMMA_K * 128) >> 4) : 2ull;
             const uint64_t b_step = p.b_mn ? (uint64_t)((UMMA_K * 128) >> 4) : 2ull;
-            uint32_t stage = 0, phase = 0, acc_phase[2] = {0, 0};
+            const uint64_t adesc0 = make_desc(a0, p.a_mn != 0), bdesc0 = make_desc(b0, p.b_mn != 0);
+            const uint32_t acc_full0 = smem_u32(&s->acc_full[0]), acc_empty0 = smem_u32(&s->acc_empty[0]);
+            uint32_t stage = 0, phase = 0;
             bool ok = true;
             int t = 0;
             for (int w = first; ok && w < n_work; w += stride, ++t) {
-                const int buf = t & 1;
+                const uint32_t buf = t & 1, use = (uint32_t)t >> 1;               // the buffer's use-th tile
                 int lo, hi;
                 slice_range(w % p.slices, lo, hi);
-                if (!(ok = wait_bar<CG>(&s->acc_empty[buf], acc_phase[buf] ^ 1, s, 2, peer_abort))) break;
+                if (!(ok = wait_bar<CG>(acc_empty0 + 8 * buf, (use & 1) ^ 1, s, 2, peer_abort))) break;
                 tc_fence_after();
-                const uint32_t d = tmem_base + (uint32_t)(buf * BN);
+                const uint32_t d = tmem_base + buf * BN;
                 for (int kb = lo; kb < hi; ++kb) {
-                    if (!(ok = wait_bar<CG>(&s->full[stage], phase, s, 3, peer_abort))) break;
+                    if (!(ok = wait_bar<CG>(full0 + 8 * stage, phase, s, 3, peer_abort))) break;
                     tc_fence_after();
-                    const uint64_t adesc = make_desc(s->a[stage], p.a_mn != 0);
-                    const uint64_t bdesc = make_desc(s->b[stage], p.b_mn != 0);
+                    const uint64_t adesc = adesc0 + stage * (C::A_STAGE >> 4), bdesc = bdesc0 + stage * (C::B_STAGE >> 4);
 #pragma unroll
                     for (int k = 0; k < BK / UMMA_K; ++k)
-                        umma<CG>(d, adesc + a_step * k, bdesc + b_step * k, idesc, (kb > lo || k) ? 1u : 0u);
-                    umma_commit<CG>(&s->empty[stage]);            // frees the slot (in both CTAs)
+                        umma_if<CG>(one, d, adesc + a_step * k, bdesc + b_step * k, idesc, (kb > lo || k) ? 1u : 0u);
+                    umma_commit_if<CG>(one, empty0 + 8 * stage);  // frees the slot (in both CTAs)
                     if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
                 }
                 if (!ok) break;
-                umma_commit<CG>(&s->acc_full[buf]);
-                acc_phase[buf] ^= 1;
+                umma_commit_if<CG>(one, acc_full0 + 8 * buf);
             }
         }
     } else {
