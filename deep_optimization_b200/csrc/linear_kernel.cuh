@@ -18,8 +18,8 @@
 //               tensor memory, two of them, so that the next tile's MMAs overlap this tile's epilogue;
 //   warps 2..9  epilogue: tcgen05.ld a 32 x 64 piece, bias, activation and its derivative, residual,
 //               one rounding, a swizzled staging buffer, a bulk tensor store of full 128-byte rows.
-//               The residual comes in through the same staging buffer by bulk tensor load, issued one
-//               piece ahead.  Outputs or residuals whose rows are not multiples of 16 bytes go through
+//               The residual comes in through the same staging buffer by bulk tensor load, asked for
+//               a tile ahead.  Outputs or residuals whose rows are not multiples of 16 bytes go through
 //               the staging buffer too and are moved by ordinary two-byte accesses.
 // A split of the reduction into slices (dW, whose reduction is the batch) writes fp32 partial tiles,
 // one plane per slice, that a second kernel adds in slice order: the result does not depend on timing.
@@ -240,43 +240,81 @@ __device__ __forceinline__ uint64_t make_desc(uint32_t tile, bool mn_major) {
 __device__ __forceinline__ float ex2_approx(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float rcp_approx(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
-// f(z) and f'(z).  GELU in its tanh form is z times the logistic function of 2u, u = k (z + c z^3):
-// one exponential and one reciprocal instruction, both within 2^-22, which a 16-bit result does not
-// show.  The polynomial sees z clamped to [-16, 16], where the logistic function is 0 or 1 to the
-// last bit, so that a huge z does not turn 0 times infinity into NaN in the derivative.
+__device__ __forceinline__ f32x2 ex2_approx2(f32x2 v) {
+    uint32_t a, b;
+    unpack2u(v, a, b);
+    return pack2(ex2_approx(__uint_as_float(a)), ex2_approx(__uint_as_float(b)));
+}
+__device__ __forceinline__ f32x2 rcp_approx2(f32x2 v) {
+    uint32_t a, b;
+    unpack2u(v, a, b);
+    return pack2(rcp_approx(__uint_as_float(a)), rcp_approx(__uint_as_float(b)));
+}
+__device__ __forceinline__ f32x2 both(float v) { return pack2(v, v); }
+
+// f(z) and f'(z) of two values, on packed fp32 pairs: as single operations the GELU with its derivative
+// took more issue slots per tile than K = 768 of MMAs last (bf16 50432 x 768 x 2304: 192 us, now 155).
+// The exponential and reciprocal instructions are within 2^-22, which a 16-bit result does not show.
+//
+// GELU in its tanh form is z times the logistic function s of 2u, u = k (z + c z^3).  z^2 is held to
+// 256 in the polynomials: beyond |z| = 16 s is 0 or 1 to the last bit whatever they say, and 0 times an
+// overflow would be NaN.
+// The exact GELU's erfc(|z| / sqrt 2) is Hastings' approximation, Abramowitz and Stegun 7.1.26 (error
+// at most 1.5e-7): a polynomial in 1 / (1 + p x) times exp(-x^2), the exponential f' needs anyway.
 template <int KIND, bool DERIV>
-__device__ __forceinline__ void activate(float z, float& y, float& d) {
+__device__ __forceinline__ void activate2(f32x2 z, f32x2& y, f32x2& d) {
     if (KIND == ACT_KIND_NONE) { y = z; return; }
-    if (KIND == ACT_KIND_RELU) { y = fmax_nan(z, 0.0f); return; }
+    if (KIND == ACT_KIND_RELU) {
+        uint32_t a, b;
+        unpack2u(z, a, b);
+        y = pack2(fmax_nan(__uint_as_float(a), 0.0f), fmax_nan(__uint_as_float(b), 0.0f));
+        return;
+    }
+    const f32x2 one = both(1.0f), minus = both(-1.0f);
     if (KIND == ACT_KIND_SILU) {
-        const float s = rcp_approx(__fadd_rn(1.0f, ex2_approx(__fmul_rn(z, -1.4426950408889634f))));
-        y = __fmul_rn(z, s);
-        if (DERIV) {
-            // y (1 - s) as z s (1 - s), with the product 0 where s is
-            const float zc = fmin_nan(fmax_nan(z, -100.0f), 100.0f);
-            d = __fmaf_rn(__fmul_rn(zc, s), __fadd_rn(1.0f, -s), s);
-        }
+        const f32x2 s = rcp_approx2(add2_rn(one, ex2_approx2(mul2_rn(z, both(-1.4426950408889634f)))));
+        y = mul2_rn(z, s);
+        if (DERIV) d = fma2_rn(y, fma2_rn(s, minus, one), s);
     }
     if (KIND == ACT_KIND_GELU) {
         constexpr float k = 0.7978845608028654f, c = 0.044715f;          // sqrt(2 / pi)
-        const float zc = fmin_nan(fmax_nan(z, -16.0f), 16.0f);
-        const float z2 = __fmul_rn(zc, zc);
-        // exp(-2u) = 2^(zc (p + q zc^2))
-        constexpr float p = -2.0f * k * 1.4426950408889634f, q = p * c;
-        const float s = rcp_approx(__fadd_rn(1.0f, ex2_approx(__fmul_rn(zc, __fmaf_rn(q, z2, p)))));
-        y = __fmul_rn(z, s);
+        constexpr float p = -2.0f * k * 1.4426950408889634f, q = p * c;  // exp(-2u) = 2^(z (p + q z^2))
+        uint32_t a, b;
+        unpack2u(mul2_rn(z, z), a, b);
+        const f32x2 z2 = pack2(fmin_nan(__uint_as_float(a), 256.0f), fmin_nan(__uint_as_float(b), 256.0f));
+        const f32x2 s = rcp_approx2(add2_rn(one, ex2_approx2(mul2_rn(z, fma2_rn(z2, both(q), both(p))))));
+        y = mul2_rn(z, s);
         if (DERIV)
-            d = __fmaf_rn(__fmul_rn(__fmul_rn(zc, s), __fadd_rn(1.0f, -s)), __fmaf_rn(6.0f * k * c, z2, 2.0f * k), s);
+            d = fma2_rn(mul2_rn(y, fma2_rn(s, minus, one)), fma2_rn(z2, both(6.0f * k * c), both(2.0f * k)), s);
     }
     if (KIND == ACT_KIND_GELU_ERF) {
-        const float cdf = __fmaf_rn(0.5f, erff(__fmul_rn(z, 0.7071067811865476f)), 0.5f);
-        y = __fmul_rn(z, cdf);
-        if (DERIV) {
-            const float zc = fmin_nan(fmax_nan(z, -16.0f), 16.0f);
-            const float pdf = __fmul_rn(0.3989422804014327f, ex2_approx(__fmul_rn(__fmul_rn(zc, zc), -0.7213475204444817f)));
-            d = __fmaf_rn(zc, pdf, cdf);
-        }
+        uint32_t a, b;
+        unpack2u(z, a, b);
+        const f32x2 size = pack2u(a & 0x7FFFFFFFu, b & 0x7FFFFFFFu);
+        const f32x2 t = rcp_approx2(fma2_rn(size, both(0.3275911f * 0.7071067811865476f), one));
+        // half of erfc's polynomial
+        f32x2 h = fma2_rn(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+        h = fma2_rn(h, t, both(0.5f * 1.421413741f));
+        h = fma2_rn(h, t, both(0.5f * -0.284496736f));
+        h = fma2_rn(h, t, both(0.5f * 0.254829592f));
+        const f32x2 e = ex2_approx2(mul2_rn(mul2_rn(z, both(-0.7213475204444817f)), z));   // exp(-z^2 / 2)
+        h = mul2_rn(mul2_rn(h, t), e);                                   // Phi(-|z|)
+        uint32_t h0, h1, u0, u1;
+        unpack2u(h, h0, h1);
+        unpack2u(fma2_rn(h, minus, one), u0, u1);
+        const f32x2 cdf = pack2u(__uint_as_float(a) >= 0.0f ? u0 : h0, __uint_as_float(b) >= 0.0f ? u1 : h1);
+        y = mul2_rn(z, cdf);
+        if (DERIV) d = fma2_rn(mul2_rn(z, e), both(0.3989422804014327f), cdf);
     }
+}
+template <int KIND, bool DERIV>
+__device__ __forceinline__ void activate(float z, float& y, float& d) {
+    f32x2 y2 = 0, d2 = 0;
+    activate2<KIND, DERIV>(both(z), y2, d2);
+    uint32_t a, b;
+    unpack2u(y2, a, b);
+    y = __uint_as_float(a);
+    if (DERIV) { unpack2u(d2, a, b); d = __uint_as_float(a); }
 }
 
 __device__ __forceinline__ float widen16(uint32_t h, int dtype) {
@@ -286,6 +324,13 @@ __device__ __forceinline__ uint32_t round_pair(float a, float b, int dtype) {
     if (dtype == ACT_DTYPE_F16) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+// the two halves of a 16-bit pair in fp32, and two fp32 rounded to such a pair
+template <int DT> __device__ __forceinline__ f32x2 widen_pair(uint32_t h) { return pack2(widen_lo<DT>(h), widen_hi<DT>(h)); }
+template <int DT> __device__ __forceinline__ uint32_t narrow_pair(f32x2 v) {
+    uint32_t a, b;
+    unpack2u(v, a, b);
+    return round_pair(__uint_as_float(a), __uint_as_float(b), DT);
 }
 __device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
     if (dtype == ACT_DTYPE_F32) return static_cast<const float*>(p)[i];
@@ -319,7 +364,7 @@ __device__ __forceinline__ void piece_in(uint8_t* buf, const unsigned short* src
 // ------------------------------------------------------------------ the kernel
 // Work item w = (tile, slice), w = (mt * n_tiles + nt) * slices + slice, dealt out round-robin to the
 // clusters: those that run together share rows of A and read all of B out of L2.
-template <int CG, int BN, int KIND, bool DERIV>
+template <int CG, int BN, int DT, int KIND, bool DERIV>
 __global__ void __launch_bounds__(THREADS, 1)
 linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
               const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_d,
@@ -413,7 +458,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         // -------------------------------------------------------------- MMA issuer (the leader's)
         if (rank == 0) {
             // fp32 accumulate; A and B f16 (0) or bf16 (1); operand majors; N / 8; M / 16
-            const uint32_t t16 = p.dtype == ACT_DTYPE_BF16 ? 1u : 0u;
+            const uint32_t t16 = DT == ACT_DTYPE_BF16 ? 1u : 0u;
             const uint32_t idesc = (1u << 4) | (t16 << 7) | (t16 << 10) | ((uint32_t)(p.a_mn != 0) << 15) | ((uint32_t)(p.b_mn != 0) << 16) |
                                    ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(C::TILE_M >> 4) << 24);
             // K = 16 further on: 32 bytes of a K-major row, or 16 rows of 128 bytes
@@ -458,7 +503,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         uint32_t full_phase[2] = {0, 0}, res_phase[2] = {0, 0};
         uint32_t seq = 0;                                         // pieces done: buffer seq & 1
         bool ok = true;
-        // the residual of this warp's piece number i of tile (m0, n0) into staging buffer b
+        // the residual of the piece at (row0, col0) into staging buffer b
         auto fetch_residual = [&](int row0, int col0, int b) {
             mbar_expect_tx(&s->res[ew][b], PIECE);
             tma_load<1>(my_stage + b * PIECE, &map_r, smem_u32(&s->res[ew][b]), col0, row0);
@@ -477,6 +522,12 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             if (!p.out_f32) {
                 if (etid < BN) s->bias[buf][etid] = p.bias && n0 + etid < p.N ? load_any(p.bias, n0 + etid, p.bias_dtype) : 0.0f;
                 asm volatile("bar.sync 1, %0;" :: "n"(EPI_WARPS * 32) : "memory");
+            }
+            if (ahead && ok && MINE == 2 && lane == 0) {
+                // the second piece's residual as early as its buffer, which the last tile's second piece
+                // left through, is free; the first one's was asked for at the end of that tile
+                tma_wait_read<0>();
+                fetch_residual(row0, n0 + (half * MINE + 1) * 64, 1);
             }
             if (ok) ok = wait_bar_warp<CG>(&s->acc_full[buf], full_phase[buf], s, 4, peer_abort);
             if (!ok) continue;
@@ -541,27 +592,22 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 #pragma unroll
                     for (int v = 0; v < 8; ++v) {
                         uint8_t* const at = yb + lane * 128 + ((v ^ (lane & 7)) << 4);
-                        float y[8], d[8];
-                        const float4 b0 = *reinterpret_cast<const float4*>(bias + v * 8), b1 = *reinterpret_cast<const float4*>(bias + v * 8 + 4);
-                        const float bb[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+                        const ulonglong2 b0 = *reinterpret_cast<const ulonglong2*>(bias + v * 8), b1 = *reinterpret_cast<const ulonglong2*>(bias + v * 8 + 4);
+                        const f32x2 bb[4] = {b0.x, b0.y, b1.x, b1.y};
+                        f32x2 y[4], d[4];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            activate<KIND, DERIV>(__fadd_rn(__uint_as_float(r[v * 8 + j]), bb[j]), y[j], d[j]);
+                        for (int j = 0; j < 4; ++j)
+                            activate2<KIND, DERIV>(add2_rn(pack2u(r[v * 8 + 2 * j], r[v * 8 + 2 * j + 1]), bb[j]), y[j], d[j]);
                         if (p.has_res) {
                             const uint4 rr = *reinterpret_cast<const uint4*>(at);
                             const uint32_t h[4] = {rr.x, rr.y, rr.z, rr.w};
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                y[2 * j] = __fadd_rn(y[2 * j], widen16(h[j] & 0xFFFFu, p.dtype));
-                                y[2 * j + 1] = __fadd_rn(y[2 * j + 1], widen16(h[j] >> 16, p.dtype));
-                            }
+                            for (int j = 0; j < 4; ++j) y[j] = add2_rn(y[j], widen_pair<DT>(h[j]));
                         }
-                        *reinterpret_cast<uint4*>(at) = make_uint4(round_pair(y[0], y[1], p.dtype), round_pair(y[2], y[3], p.dtype),
-                                                                   round_pair(y[4], y[5], p.dtype), round_pair(y[6], y[7], p.dtype));
+                        *reinterpret_cast<uint4*>(at) = make_uint4(narrow_pair<DT>(y[0]), narrow_pair<DT>(y[1]), narrow_pair<DT>(y[2]), narrow_pair<DT>(y[3]));
                         if (DERIV)
                             *reinterpret_cast<uint4*>(my_stage + PIECE + lane * 128 + ((v ^ (lane & 7)) << 4)) =
-                                make_uint4(round_pair(d[0], d[1], p.dtype), round_pair(d[2], d[3], p.dtype),
-                                           round_pair(d[4], d[5], p.dtype), round_pair(d[6], d[7], p.dtype));
+                                make_uint4(narrow_pair<DT>(d[0]), narrow_pair<DT>(d[1]), narrow_pair<DT>(d[2]), narrow_pair<DT>(d[3]));
                     }
                     if (p.tma_out) {
                         // the 32 x 64 piece leaves as one bulk tensor store, clipped at the tensor's edges
@@ -573,16 +619,12 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                                 if (DERIV) tma_store_2d(&map_d, my_stage + PIECE, col0, row0);
                             }
                             tma_commit();                         // also when nothing was stored: the groups count pieces
-                            if (ahead) {
-                                // the next piece's residual goes into the other buffer once its last store has read it
-                                int nw = w, ni = i + 1;
-                                if (ni == MINE) { ni = 0; nw += stride; }
-                                if (ok && nw < n_work) {
-                                    const int nt = nw / p.slices;
-                                    tma_wait_read<1>();
-                                    fetch_residual((nt / n_tiles) * C::TILE_M + (int)rank * BM + q * 32,
-                                                   (nt % n_tiles) * BN + (half * MINE + ni) * 64, b ^ 1);
-                                }
+                            if (ahead && i == MINE - 1 && ok && w + stride < n_work) {
+                                // the next tile's first residual goes into the other buffer once its store has read it
+                                const int nt = (w + stride) / p.slices;
+                                tma_wait_read<1>();
+                                fetch_residual((nt / n_tiles) * C::TILE_M + (int)rank * BM + q * 32,
+                                               (nt % n_tiles) * BN + half * MINE * 64, b ^ 1);
                             }
                         }
                     } else {
@@ -622,9 +664,9 @@ template <int CG, int BN> bool launch_kernel(int kind, bool deriv, const Maps& m
 // the abort reason of that file's kernels on the current device; synchronises
 template <int CG, int BN> bool kernel_error(unsigned int* out, bool clear);
 
-template <int CG, int BN, int KIND, bool DERIV>
+template <int CG, int BN, int DT, int KIND, bool DERIV>
 bool launch_one(const Maps& m, const Params& p, int grid, cudaStream_t st) {
-    auto* k = linear_kernel<CG, BN, KIND, DERIV>;
+    auto* k = linear_kernel<CG, BN, DT, KIND, DERIV>;
     const int smem = (int)sizeof(Smem<CG, BN>);
     // the shared-memory opt-in is an attribute of the kernel on each device: set on the first launch there
     static bool ready[64];
@@ -648,18 +690,22 @@ bool launch_one(const Maps& m, const Params& p, int grid, cudaStream_t st) {
 
 // instantiated once per tile shape, in a file of its own so that they compile in parallel
 #define ACT_LINEAR_INSTANTIATE(CG, BN)                                                                                   \
-    template <> bool launch_kernel<CG, BN>(int kind, bool deriv, const Maps& m, const Params& p, int grid, cudaStream_t st) { \
+    template <int DT> bool launch_kind(int kind, bool deriv, const Maps& m, const Params& p, int grid, cudaStream_t st) { \
         switch (kind) {                                                                                                  \
-            case ACT_KIND_NONE: return launch_one<CG, BN, ACT_KIND_NONE, false>(m, p, grid, st);                         \
-            case ACT_KIND_RELU: return launch_one<CG, BN, ACT_KIND_RELU, false>(m, p, grid, st);                         \
-            case ACT_KIND_GELU: return deriv ? launch_one<CG, BN, ACT_KIND_GELU, true>(m, p, grid, st)                   \
-                                             : launch_one<CG, BN, ACT_KIND_GELU, false>(m, p, grid, st);                 \
-            case ACT_KIND_SILU: return deriv ? launch_one<CG, BN, ACT_KIND_SILU, true>(m, p, grid, st)                   \
-                                             : launch_one<CG, BN, ACT_KIND_SILU, false>(m, p, grid, st);                 \
-            case ACT_KIND_GELU_ERF: return deriv ? launch_one<CG, BN, ACT_KIND_GELU_ERF, true>(m, p, grid, st)           \
-                                                 : launch_one<CG, BN, ACT_KIND_GELU_ERF, false>(m, p, grid, st);         \
+            case ACT_KIND_NONE: return launch_one<CG, BN, DT, ACT_KIND_NONE, false>(m, p, grid, st);                     \
+            case ACT_KIND_RELU: return launch_one<CG, BN, DT, ACT_KIND_RELU, false>(m, p, grid, st);                     \
+            case ACT_KIND_GELU: return deriv ? launch_one<CG, BN, DT, ACT_KIND_GELU, true>(m, p, grid, st)               \
+                                             : launch_one<CG, BN, DT, ACT_KIND_GELU, false>(m, p, grid, st);             \
+            case ACT_KIND_SILU: return deriv ? launch_one<CG, BN, DT, ACT_KIND_SILU, true>(m, p, grid, st)               \
+                                             : launch_one<CG, BN, DT, ACT_KIND_SILU, false>(m, p, grid, st);             \
+            case ACT_KIND_GELU_ERF: return deriv ? launch_one<CG, BN, DT, ACT_KIND_GELU_ERF, true>(m, p, grid, st)       \
+                                                 : launch_one<CG, BN, DT, ACT_KIND_GELU_ERF, false>(m, p, grid, st);     \
             default: return false;                                                                                       \
         }                                                                                                                \
+    }                                                                                                                    \
+    template <> bool launch_kernel<CG, BN>(int kind, bool deriv, const Maps& m, const Params& p, int grid, cudaStream_t st) { \
+        return p.dtype == ACT_DTYPE_BF16 ? launch_kind<ACT_DTYPE_BF16>(kind, deriv, m, p, grid, st)                      \
+                                         : launch_kind<ACT_DTYPE_F16>(kind, deriv, m, p, grid, st);                      \
     }                                                                                                                    \
     template <> bool kernel_error<CG, BN>(unsigned int* out, bool clear) {                                               \
         const unsigned int zero = 0;                                                                                     \
