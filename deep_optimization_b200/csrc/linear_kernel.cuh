@@ -147,7 +147,6 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
 }
 __device__ __forceinline__ void tma_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 template <int KEEP> __device__ __forceinline__ void tma_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" :: "n"(KEEP) : "memory"); }
-__device__ __forceinline__ void tma_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 template <int CG> __device__ __forceinline__ void tmem_alloc(uint32_t* dst_smem) {
     if (CG == 2) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(dst_smem)), "n"(TMEM_COLS) : "memory");
@@ -403,6 +402,8 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     sync_all<CG>();                                               // barriers of both CTAs exist from here on
     tc_fence_after();
     const uint32_t tmem_base = s->tmem_base;
+    grid_dependency_wait();                                       // from here on global memory is touched
+    grid_launch_dependents();
 
     // blocks [lo, hi) of the reduction belong to slice sl
     auto slice_range = [&](int sl, int& lo, int& hi) {
@@ -570,28 +571,20 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     // y (and the residual) in buffer b; the derivative in buffer 1 when there is one
                     const int b = DERIV ? 0 : (int)(seq & 1);
                     uint8_t* const yb = my_stage + b * PIECE;
-                    if (ahead) {
-                        ok = wait_bar_warp<CG>(&s->res[ew][b], res_phase[b], s, 7, peer_abort);
-                        res_phase[b] ^= 1;
-                    } else {
-                        // the store that last read this buffer is done with it
-                        if (p.tma_out && lane == 0) { if (DERIV) tma_wait_read<0>(); else tma_wait_read<1>(); }
-                        __syncwarp();
-                        if (p.has_res) {
-                            if (p.tma_out) {
-                                if (lane == 0) fetch_residual(row0, col0, b);
-                                ok = wait_bar_warp<CG>(&s->res[ew][b], res_phase[b], s, 7, peer_abort);
-                                res_phase[b] ^= 1;
-                            } else {
-                                piece_in(yb, static_cast<const unsigned short*>(p.res) + (int64_t)row0 * p.ld_res + col0, p.ld_res, rows, p.N - col0, lane);
-                                __syncwarp();
-                            }
+                    if (p.has_res) {
+                        if (p.tma_out) {
+                            if (!ahead && lane == 0) { tma_wait_read<0>(); fetch_residual(row0, col0, b); }
+                            ok = wait_bar_warp<CG>(&s->res[ew][b], res_phase[b], s, 7, peer_abort);
+                            res_phase[b] ^= 1;
+                        } else {
+                            piece_in(yb, static_cast<const unsigned short*>(p.res) + (int64_t)row0 * p.ld_res + col0, p.ld_res, rows, p.N - col0, lane);
+                            __syncwarp();
                         }
                     }
                     const float* const bias = s->bias[buf] + (half * MINE + i) * 64;
+                    // r[8 v ..]: eight columns of z become four words of y and four of the derivative
 #pragma unroll
                     for (int v = 0; v < 8; ++v) {
-                        uint8_t* const at = yb + lane * 128 + ((v ^ (lane & 7)) << 4);
                         const ulonglong2 b0 = *reinterpret_cast<const ulonglong2*>(bias + v * 8), b1 = *reinterpret_cast<const ulonglong2*>(bias + v * 8 + 4);
                         const f32x2 bb[4] = {b0.x, b0.y, b1.x, b1.y};
                         f32x2 y[4], d[4];
@@ -599,15 +592,29 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         for (int j = 0; j < 4; ++j)
                             activate2<KIND, DERIV>(add2_rn(pack2u(r[v * 8 + 2 * j], r[v * 8 + 2 * j + 1]), bb[j]), y[j], d[j]);
                         if (p.has_res) {
-                            const uint4 rr = *reinterpret_cast<const uint4*>(at);
+                            const uint4 rr = *reinterpret_cast<const uint4*>(yb + lane * 128 + ((v ^ (lane & 7)) << 4));
                             const uint32_t h[4] = {rr.x, rr.y, rr.z, rr.w};
 #pragma unroll
                             for (int j = 0; j < 4; ++j) y[j] = add2_rn(y[j], widen_pair<DT>(h[j]));
                         }
-                        *reinterpret_cast<uint4*>(at) = make_uint4(narrow_pair<DT>(y[0]), narrow_pair<DT>(y[1]), narrow_pair<DT>(y[2]), narrow_pair<DT>(y[3]));
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            r[v * 8 + j] = narrow_pair<DT>(y[j]);
+                            if (DERIV) r[v * 8 + 4 + j] = narrow_pair<DT>(d[j]);
+                        }
+                    }
+                    // the stores that last read the buffers are done with them (a residual's own buffer was free before)
+                    if (p.tma_out && lane == 0) {
+                        if (DERIV) tma_wait_read<0>();
+                        else if (!p.has_res) tma_wait_read<1>();
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int v = 0; v < 8; ++v) {
+                        const int at = lane * 128 + ((v ^ (lane & 7)) << 4);
+                        *reinterpret_cast<uint4*>(yb + at) = make_uint4(r[v * 8], r[v * 8 + 1], r[v * 8 + 2], r[v * 8 + 3]);
                         if (DERIV)
-                            *reinterpret_cast<uint4*>(my_stage + PIECE + lane * 128 + ((v ^ (lane & 7)) << 4)) =
-                                make_uint4(narrow_pair<DT>(d[0]), narrow_pair<DT>(d[1]), narrow_pair<DT>(d[2]), narrow_pair<DT>(d[3]));
+                            *reinterpret_cast<uint4*>(my_stage + PIECE + at) = make_uint4(r[v * 8 + 4], r[v * 8 + 5], r[v * 8 + 6], r[v * 8 + 7]);
                     }
                     if (p.tma_out) {
                         // the 32 x 64 piece leaves as one bulk tensor store, clipped at the tensor's edges
@@ -642,7 +649,7 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 mbar_arrive_cluster(map_to_cta(smem_u32(&s->acc_empty[buf]), 0));
             }
         }
-        if (lane == 0) tma_wait_all();                            // all of this warp's stores are complete before exit
+        if (lane == 0) tma_wait_read<0>();                        // the staging buffers are read before the CTA leaves
     }
 
     __syncwarp();                                                 // lanes that had no role wait for the one that had
@@ -681,10 +688,12 @@ bool launch_one(const Maps& m, const Params& p, int grid, cudaStream_t st) {
     cfg.blockDim = dim3(THREADS, 1, 1);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = CG == 2 ? 1 : 0;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CG; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = CG == 2 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, k, m.a, m.b, m.y, m.d, m.r, p) == cudaSuccess;
 }
 
