@@ -84,18 +84,25 @@ few_rows_kernel(const unsigned short* __restrict__ x, int64_t ld_x, const unsign
     if (d) d[lane * ld_d + n] = (unsigned short)round_pair(dv, 0.0f, dtype);
 }
 
-// rows of 16-bit elements copied to a pitch that a bulk tensor copy can read (a multiple of 16 bytes)
+// Rows of 16-bit elements copied to a pitch that a bulk tensor copy can read (a multiple of 16 bytes):
+// all operands of a call that need it in one launch.
+struct PadJob { const unsigned short* src; unsigned short* dst; int64_t ld, ld_dst, end; int cols; };   // end: 16-byte pieces up to here
+struct PadJobs { PadJob job[3]; };
+
 __global__ void __launch_bounds__(256)
-pad_rows_kernel(const unsigned short* __restrict__ src, int64_t ld, int64_t rows, int cols, unsigned short* __restrict__ dst, int64_t ld_dst)
+pad_rows_kernel(const __grid_constant__ PadJobs jobs)
 {
-    const int64_t pieces = ld_dst >> 3;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < rows * pieces; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t r = i / pieces;
-        const int c = (int)(i - r * pieces) * 8;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < jobs.job[2].end; i += (int64_t)gridDim.x * blockDim.x) {
+        const int k = i < jobs.job[0].end ? 0 : (i < jobs.job[1].end ? 1 : 2);
+        const PadJob& j = jobs.job[k];
+        const int64_t at = k ? i - jobs.job[k - 1].end : i, pieces = j.ld_dst >> 3;
+        const int64_t r = at >> 32 ? at / pieces : (int64_t)((uint32_t)at / (uint32_t)pieces);
+        const int c = (int)(at - r * pieces) * 8;
+        const unsigned short* src = j.src + r * j.ld + c;
         uint32_t h[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = c + j < cols ? __ldg(src + r * ld + c + j) : 0u;
-        *reinterpret_cast<uint4*>(dst + r * ld_dst + c) = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+        for (int e = 0; e < 8; ++e) h[e] = c + e < j.cols ? __ldg(src + e) : 0u;
+        *reinterpret_cast<uint4*>(j.dst + r * j.ld_dst + c) = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
     }
 }
 
@@ -137,11 +144,13 @@ sum_slices_kernel(const float* __restrict__ part, int64_t ld_part, int64_t plane
 // every time.  Bound: HBM, dy and d read once, dz written once.
 constexpr int kMulThreads = 256;
 
-template <int V>
+// W 32-bit words (2 W elements) per access, or one element (W = 0); ROWS rows' loads in flight
+template <int W>
 __global__ void __launch_bounds__(kMulThreads)
 mul_col_sum_kernel(const unsigned short* __restrict__ dy, const unsigned short* __restrict__ d, unsigned short* __restrict__ dz,
                    float* __restrict__ part, int64_t M, int N, int dtype, int tpr)
 {
+    constexpr int V = W ? 2 * W : 1, ROWS = 4;
     __shared__ float sums[kMulThreads * V];
     const int rpi = kMulThreads / tpr;                       // rows per step of the block
     const int ql = threadIdx.x % tpr, rl = threadIdx.x / tpr;
@@ -151,30 +160,45 @@ mul_col_sum_kernel(const unsigned short* __restrict__ dy, const unsigned short* 
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.0f;
     if (rl < rpi && c < N) {
-        if (V == 8) {
-#pragma unroll 4
-            for (int64_t r = r0 + rl; r < r1; r += rpi) {
-                const int64_t at = r * N + c;
-                const uint4 a = ldg_stream_v4(dy + at), b = ldg_stream_v4(d + at);
-                const uint32_t ua[4] = {a.x, a.y, a.z, a.w}, ub[4] = {b.x, b.y, b.z, b.w};
-                uint32_t o[4];
+        for (int64_t r = r0 + rl; r < r1; r += ROWS * rpi) {
+            if (W) {
+                uint4 a[ROWS], b[ROWS];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float lo = __fmul_rn(widen16(ua[i] & 0xFFFFu, dtype), widen16(ub[i] & 0xFFFFu, dtype));
-                    const float hi = __fmul_rn(widen16(ua[i] >> 16, dtype), widen16(ub[i] >> 16, dtype));
-                    acc[(2 * i) % V] = __fadd_rn(acc[(2 * i) % V], lo);
-                    acc[(2 * i + 1) % V] = __fadd_rn(acc[(2 * i + 1) % V], hi);
-                    o[i] = round_pair(lo, hi, dtype);
+                for (int u = 0; u < ROWS; ++u)
+                    if (r + u * rpi < r1) {
+                        a[u] = ldg_stream_v4(dy + (r + u * rpi) * N + c);
+                        b[u] = ldg_stream_v4(d + (r + u * rpi) * N + c);
+                    }
+#pragma unroll
+                for (int u = 0; u < ROWS; ++u) {
+                    if (r + u * rpi >= r1) break;
+                    const uint32_t ua[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, ub[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
+                    uint32_t o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float lo = __fmul_rn(widen16(ua[i] & 0xFFFFu, dtype), widen16(ub[i] & 0xFFFFu, dtype));
+                        const float hi = __fmul_rn(widen16(ua[i] >> 16, dtype), widen16(ub[i] >> 16, dtype));
+                        acc[(2 * i) % V] = __fadd_rn(acc[(2 * i) % V], lo);
+                        acc[(2 * i + 1) % V] = __fadd_rn(acc[(2 * i + 1) % V], hi);
+                        o[i] = round_pair(lo, hi, dtype);
+                    }
+                    stg_stream_v4(dz + (r + u * rpi) * N + c, make_uint4(o[0], o[1], o[2], o[3]));
                 }
-                *reinterpret_cast<uint4*>(dz + at) = make_uint4(o[0], o[1], o[2], o[3]);
-            }
-        } else {
-#pragma unroll 4
-            for (int64_t r = r0 + rl; r < r1; r += rpi) {
-                const int64_t at = r * N + c;
-                const float v = __fmul_rn(widen16(__ldg(dy + at), dtype), widen16(__ldg(d + at), dtype));
-                acc[0] = __fadd_rn(acc[0], v);
-                dz[at] = (unsigned short)round_pair(v, 0.0f, dtype);
+            } else {
+                float va[ROWS], vb[ROWS];
+#pragma unroll
+                for (int u = 0; u < ROWS; ++u)
+                    if (r + u * rpi < r1) {
+                        va[u] = widen16(__ldg(dy + (r + u * rpi) * N + c), dtype);
+                        vb[u] = widen16(__ldg(d + (r + u * rpi) * N + c), dtype);
+                    }
+#pragma unroll
+                for (int u = 0; u < ROWS; ++u) {
+                    if (r + u * rpi >= r1) break;
+                    const float v = __fmul_rn(va[u], vb[u]);
+                    acc[0] = __fadd_rn(acc[0], v);
+                    dz[(r + u * rpi) * N + c] = (unsigned short)round_pair(v, 0.0f, dtype);
+                }
             }
         }
     }
@@ -267,14 +291,17 @@ size_t pad_bytes(const Mat& m) { return tma_ready(m) ? 0 : align256((size_t)m.ro
 
 struct Plan { int variant; int slices; };
 
-// Tile shape and split of the reduction.  The model is waves * (k blocks * cycles a block + cycles a
-// tile), the cycles measured per shape (see the table in choose()).
+// Tile shape and split of the reduction, by a model of the time in microseconds: a start, then waves of
+// (64-deep blocks of the reduction + the tile's own cost).  Measured at K = 768, N = 768 to 2304, both sides
+// of each choice: [197, 768] x [768, 768] 8.2 us with pairs, 6.3 with 128 x 128 tiles, 5.7 with 128 x 64;
+// [1024, 768] x [768, 2304] 8.8, 7.1, 9.4; [6304, 768] x [768, 2304] 20.2, 25.1, 39.5.
+// Partial planes (the split) cost their bytes, written and read at L2's pace, and one more launch.
 Plan choose(int64_t M, int64_t N, int64_t K, bool may_slice, int variant) {
     const int sms = act::stream_grid_for((int64_t)1 << 40, 1, 1);
-    struct Shape { int id; int tm, tn, units; double per_block, per_tile; };
-    const Shape shapes[3] = {{ACT_LINEAR_PAIR, 256, 256, sms / 2 < 1 ? 1 : sms / 2, 540.0, 2600.0},
-                             {ACT_LINEAR_128, 128, 128, sms, 420.0, 1800.0},
-                             {ACT_LINEAR_64, 128, 64, sms, 330.0, 1400.0}};
+    struct Shape { int id; int tm, tn, units; double start, per_block, per_tile; };
+    const Shape shapes[3] = {{ACT_LINEAR_PAIR, 256, 256, sms / 2 < 1 ? 1 : sms / 2, 3.7, 0.27, 0.5},
+                             {ACT_LINEAR_128, 128, 128, sms, 2.8, 0.225, 0.3},
+                             {ACT_LINEAR_64, 128, 64, sms, 2.7, 0.18, 0.2}};
     const int64_t kb = ceil_div(K, BK);
     Plan best = {ACT_LINEAR_PAIR, 1};
     double best_cost = 1e300;
@@ -282,27 +309,35 @@ Plan choose(int64_t M, int64_t N, int64_t K, bool may_slice, int variant) {
         if (variant && s.id != variant) continue;
         const int64_t tiles = ceil_div(M, s.tm) * ceil_div(N, s.tn);
         for (int sl = 1; sl <= (may_slice ? 148 : 1) && sl <= kb; ++sl) {
-            // partial planes stay within 64 MB, so that they live in L2
+            // a slice is at least four blocks deep, the planes stay within 64 MB, so that they live in L2
             if (sl > 1 && ((double)sl * M * N * 4 > 64e6 || kb / sl < 4)) break;
             const double waves = (double)ceil_div(tiles * sl, s.units);
-            double cost = waves * ((double)ceil_div(kb, sl) * s.per_block + s.per_tile);
-            if (may_slice) cost += 4000.0 + (double)(sl + 1) * M * N * 4 / 3000.0;
+            double cost = s.start + waves * ((double)ceil_div(kb, sl) * s.per_block + s.per_tile);
+            if (sl > 1) cost += 2.5 + (double)(2 * sl + 1) * M * N * 4 / 6e6;
             if (cost < best_cost) { best_cost = cost; best = {s.id, sl}; }
         }
     }
     return best;
 }
 
-int pad_rows(Mat& m, uint8_t*& ws, cudaStream_t st) {
-    if (tma_ready(m)) return ACT_OK;
-    const int64_t ld = round_up(m.cols, 8);
-    const int64_t blocks = ceil_div(m.rows * (ld / 8), 256);
-    pad_rows_kernel<<<act::stream_grid_for(blocks, 8, 4), 256, 0, st>>>(static_cast<const unsigned short*>(m.p), m.ld, m.rows,
-                                                                    (int)m.cols, reinterpret_cast<unsigned short*>(ws), ld);
-    if (cudaGetLastError() != cudaSuccess) return ACT_ERR_LAUNCH;
-    ws += pad_bytes(m);
-    m = Mat{ws - align256((size_t)m.rows * (size_t)ld * 2), ld, m.rows, m.cols};
-    return ACT_OK;
+// copies those of the n operands that a bulk copy cannot read into the workspace, moving ws on
+int pad_rows(Mat* const* mats, int n, uint8_t*& ws, cudaStream_t st) {
+    PadJobs jobs = {};
+    int64_t end = 0;
+    int k = 0;
+    for (int i = 0; i < n; ++i) {
+        Mat& m = *mats[i];
+        if (tma_ready(m)) continue;
+        const int64_t ld = round_up(m.cols, 8);
+        end += m.rows * (ld / 8);
+        jobs.job[k++] = PadJob{static_cast<const unsigned short*>(m.p), reinterpret_cast<unsigned short*>(ws), m.ld, ld, end, (int)m.cols};
+        m = Mat{ws, ld, m.rows, m.cols};
+        ws += align256((size_t)m.rows * (size_t)ld * 2);
+    }
+    if (k == 0) return ACT_OK;
+    for (; k < 3; ++k) jobs.job[k].end = end;
+    pad_rows_kernel<<<act::stream_grid_for(ceil_div(end, 256), 8, 4), 256, 0, st>>>(jobs);
+    return cudaGetLastError() == cudaSuccess ? ACT_OK : ACT_ERR_LAUNCH;
 }
 
 // C [M, N] = A B^T in p's epilogue; a and b as stored (K-major: rows of the output index; MN-major: rows
@@ -389,8 +424,8 @@ extern "C" int act_linear_fwd(const void* x, int64_t ld_x, const void* w, int64_
     if (need && (!workspace || ws_bytes < need)) return ACT_ERR_WORKSPACE;
     if (need && ((uintptr_t)workspace & 15)) return ACT_ERR_ALIGN;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    int rc = pad_rows(a, ws, st);
-    if (rc == ACT_OK) rc = pad_rows(b, ws, st);
+    Mat* const operands[2] = {&a, &b};
+    const int rc = pad_rows(operands, 2, ws, st);
     if (rc != ACT_OK) return rc;
     Params p = {};
     p.M = M; p.N = N; p.K = K; p.slices = 1; p.dtype = dtype;
@@ -432,29 +467,30 @@ extern "C" int act_linear_bwd(const void* dz, int64_t ld_dz, const void* x, int6
     if (need && ((uintptr_t)workspace & 15)) return ACT_ERR_ALIGN;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    Mat g = {dz, ld_dz, M, N};
-    int rc = pad_rows(g, ws, st);
+    Mat g = {dz, ld_dz, M, N}, wm = {w, ld_w, N, K}, xm = {x, ld_x, M, K};
+    Mat* operands[3];
+    int n = 0;
+    operands[n++] = &g;
+    if (dx) operands[n++] = &wm;
+    if (dw) operands[n++] = &xm;
+    int rc = pad_rows(operands, n, ws, st);
     if (rc != ACT_OK) return rc;
     if (dx) {
         // dx[m, k] = sum_n dz[m, n] W[n, k]: dz K-major, W MN-major
-        Mat b = {w, ld_w, N, K};
-        if ((rc = pad_rows(b, ws, st)) != ACT_OK) return rc;
         Params p = {};
         p.M = M; p.N = K; p.K = N; p.b_mn = 1; p.slices = 1; p.dtype = dtype;
         p.y = dx; p.ld_y = ld_dx; p.tma_out = tensor_ready(dx, ld_dx);
-        if ((rc = launch(g, b, p, choose(M, K, N, false, variant).variant, ACT_KIND_NONE, false, st)) != ACT_OK) return rc;
+        if ((rc = launch(g, wm, p, choose(M, K, N, false, variant).variant, ACT_KIND_NONE, false, st)) != ACT_OK) return rc;
     }
     if (dw) {
         // dW[n, k] = sum_m dz[m, n] x[m, k]: both MN-major, the reduction is the batch
-        Mat b = {x, ld_x, M, K};
-        if ((rc = pad_rows(b, ws, st)) != ACT_OK) return rc;
         const Plan plan = choose(N, K, M, true, variant);
         Params p = {};
         p.M = N; p.N = K; p.K = M; p.a_mn = p.b_mn = 1; p.slices = plan.slices; p.dtype = dtype;
         const bool planes = plan.slices > 1 || dw_dtype == ACT_DTYPE_F32;
         if (planes) { p.out_f32 = 1; p.y = ws; p.ld_y = round_up(K, 4); }
         else { p.y = dw; p.ld_y = ld_dw; p.tma_out = tensor_ready(dw, ld_dw); }
-        if ((rc = launch(g, b, p, plan.variant, ACT_KIND_NONE, false, st)) != ACT_OK) return rc;
+        if ((rc = launch(g, xm, p, plan.variant, ACT_KIND_NONE, false, st)) != ACT_OK) return rc;
         if (planes) {
             const int64_t blocks = ceil_div((int64_t)N * (p.ld_y / 4), 256);
             sum_slices_kernel<<<act::stream_grid_for(blocks, 8, 4), 256, 0, st>>>(
@@ -515,8 +551,8 @@ extern "C" int act_mul_col_sum(const void* dy, const void* d, int dtype, int64_t
     auto* o = static_cast<unsigned short*>(dz);
     float* part = db ? static_cast<float*>(workspace) : nullptr;
     const dim3 grid((unsigned)gx, (unsigned)gy);
-    if (vec) mul_col_sum_kernel<8><<<grid, kMulThreads, 0, st>>>(a, b, o, part, M, N, dtype, tpr);
-    else mul_col_sum_kernel<1><<<grid, kMulThreads, 0, st>>>(a, b, o, part, M, N, dtype, tpr);
+    if (vec) mul_col_sum_kernel<4><<<grid, kMulThreads, 0, st>>>(a, b, o, part, M, N, dtype, tpr);
+    else mul_col_sum_kernel<0><<<grid, kMulThreads, 0, st>>>(a, b, o, part, M, N, dtype, tpr);
     if (cudaGetLastError() != cudaSuccess) return ACT_ERR_LAUNCH;
     if (db) {
         col_sum_slices_kernel<<<(unsigned)ceil_div(N, 32), 1024, 0, st>>>(part, gy, N, db);

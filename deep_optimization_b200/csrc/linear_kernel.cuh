@@ -11,12 +11,12 @@
 // tcgen05.mma.cta_group::2 (each CTA stages its own 128 rows of A and its own half of B, and keeps the
 // accumulators of its own rows in its own tensor memory).  CG = 1: one CTA per 128 x BN tile, for
 // problems with too few rows or columns to fill the GPU with pairs.
-// Roles of a CTA's 320 threads:
+// Roles of a CTA's warps:
 //   warp 0      TMA producer: 64 k of both operands per stage, as rows of 128 bytes with the 128-byte
 //               swizzle, completion counted on the leader's barrier (no multicast);
 //   warp 1      MMA issuer (the leader's): four tcgen05.mma of K = 16 per stage, fp32 accumulators in
 //               tensor memory, two of them, so that the next tile's MMAs overlap this tile's epilogue;
-//   warps 2..9  epilogue: tcgen05.ld a 32 x 64 piece, bias, activation and its derivative, residual,
+//   warps 2..   epilogue (eight, four for 64 columns): tcgen05.ld a 32 x 64 piece, bias, activation and its derivative, residual,
 //               one rounding, a swizzled staging buffer, a bulk tensor store of full 128-byte rows.
 //               The residual comes in through the same staging buffer by bulk tensor load, asked for
 //               a tile ahead.  Outputs or residuals whose rows are not multiples of 16 bytes go through
@@ -38,8 +38,6 @@ constexpr int BM = 128;                         // rows of A per CTA
 constexpr int BK = 64;                          // reduction per stage: 128 bytes of a 16-bit type
 constexpr int UMMA_K = 16;
 constexpr int CHUNK = BK * 128;                 // MN-major: 64 columns x BK rows
-constexpr int EPI_WARPS = 8;
-constexpr int THREADS = 64 + EPI_WARPS * 32;
 constexpr int PIECE = 32 * 128;                 // staging buffer: 32 rows of 128 bytes
 constexpr int TMEM_COLS = 512;
 constexpr uint32_t SPIN_LIMIT = 1u << 24;
@@ -47,17 +45,19 @@ constexpr uint32_t SPIN_LIMIT = 1u << 24;
 template <int CG, int BN> struct Cfg {
     static constexpr int BNC = BN / CG;                          // rows of B per CTA
     static constexpr int A_STAGE = BM * 128, B_STAGE = BNC * 128;
-    // what the 64 KB of staging buffers leave of an SM's 227 KB
-    static constexpr int STAGES = BNC == 128 ? 5 : 6;
+    // a warp drains 32 rows of a tile's left or right half, or of all 64 columns
+    static constexpr int EPI_WARPS = BN == 64 ? 4 : 8, THREADS = 64 + EPI_WARPS * 32;
+    // what two 4 KB staging buffers per epilogue warp leave of an SM's 227 KB
+    static constexpr int STAGES = BNC == 128 ? 5 : 8;
     static constexpr int TILE_M = BM * CG;
 };
 
 template <int CG, int BN> struct __align__(1024) Smem {
     uint8_t a[Cfg<CG, BN>::STAGES][Cfg<CG, BN>::A_STAGE];
     uint8_t b[Cfg<CG, BN>::STAGES][Cfg<CG, BN>::B_STAGE];
-    uint8_t stage[EPI_WARPS][2][PIECE];          // 128-byte rows, 16-byte pieces xor-swizzled by row & 7
+    uint8_t stage[Cfg<CG, BN>::EPI_WARPS][2][PIECE];          // 128-byte rows, 16-byte pieces xor-swizzled by row & 7
     float bias[2][BN];
-    uint64_t full[Cfg<CG, BN>::STAGES], empty[Cfg<CG, BN>::STAGES], acc_full[2], acc_empty[2], res[EPI_WARPS][2];
+    uint64_t full[Cfg<CG, BN>::STAGES], empty[Cfg<CG, BN>::STAGES], acc_full[2], acc_empty[2], res[Cfg<CG, BN>::EPI_WARPS][2];
     uint32_t tmem_base;
     volatile uint32_t abort;
 };
@@ -83,8 +83,8 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)_
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(smem_u32(bar)), "r"(count));
 }
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(smem_u32(bar)), "r"(bytes) : "memory");
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -112,31 +112,22 @@ template <int CG> __device__ __forceinline__ void sync_all() {
 __device__ __forceinline__ void fence_barrier_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // operand load; the bytes are counted on the leader's barrier (`bar`: its cluster address)
-// (`dst`: its shared-memory address; `on`: whether this thread issues it)
-template <int CG> __device__ __forceinline__ void tma_load_if(uint32_t on, uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
-    if (CG == 2)
-        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t"
-                     "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
-                     :: "r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(on) : "memory");
-    else
-        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t"
-                     "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
-                     :: "r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(on) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx_if(uint32_t on, uint32_t bar, uint32_t bytes) {
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}"
-                 :: "r"(bar), "r"(bytes), "r"(on) : "memory");
-}
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" :: "l"(map) : "memory"); }
-// residual load, one CTA's own
-template <int CG> __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+// (`dst`: its shared-memory address)
+template <int CG> __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
     if (CG == 2)
         asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                     :: "r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+                     :: "r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
     else
         asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                     :: "r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+                     :: "r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
 }
+// true in one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(e));
+    return e != 0;
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" :: "l"(map) : "memory"); }
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
                  :: "l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1) : "memory");
@@ -162,23 +153,21 @@ template <int CG> __device__ __forceinline__ void tmem_dealloc(uint32_t taddr) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-template <int CG> __device__ __forceinline__ void umma_if(uint32_t on, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+template <int CG> __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     if (CG == 2)
-        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                     :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
     else
-        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                     :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
 // arrives, once the MMAs issued so far are done, on the barrier at this offset (in both CTAs of a pair)
-template <int CG> __device__ __forceinline__ void umma_commit_if(uint32_t on, uint32_t bar) {
+template <int CG> __device__ __forceinline__ void umma_commit(uint32_t bar) {
     if (CG == 2) {
         const uint16_t both = 3;
-        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
-                     :: "r"(bar), "h"(both), "r"(on) : "memory");
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" :: "r"(bar), "h"(both) : "memory");
     } else {
-        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
-                     :: "r"(bar), "r"(on) : "memory");
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
     }
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
@@ -194,7 +183,8 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // A wait that runs out records why and raises this CTA's abort flag and its peer's.  Every lane of the
-// warp waits, so that the loops around it stay uniform over the warp.
+// warp waits, so that the loops around it stay uniform over the warp (one lane's wait and a broadcast of
+// its outcome took 130 cycles more per stage).
 template <int CG, typename S>
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, S* s, uint32_t code, uint32_t peer_abort) {
     bool ok = mbar_try_wait(bar, parity);
@@ -364,13 +354,14 @@ __device__ __forceinline__ void piece_in(uint8_t* buf, const unsigned short* src
 // Work item w = (tile, slice), w = (mt * n_tiles + nt) * slices + slice, dealt out round-robin to the
 // clusters: those that run together share rows of A and read all of B out of L2.
 template <int CG, int BN, int DT, int KIND, bool DERIV>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Cfg<CG, BN>::THREADS, 1)
 linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
               const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_d,
               const __grid_constant__ CUtensorMap map_r, const __grid_constant__ Params p)
 {
     using C = Cfg<CG, BN>;
     using S = Smem<CG, BN>;
+    constexpr int EPI_WARPS = C::EPI_WARPS;
     extern __shared__ __align__(1024) uint8_t smem_raw_linear[];
     S* s = reinterpret_cast<S*>(smem_raw_linear);
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform, and known to be
@@ -412,11 +403,13 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         hi = lo + per + (sl < extra ? 1 : 0);
     };
 
-    // The producer's and the issuer's loops run on a whole warp, uniform over it, and one lane's
-    // predicate guards each load, MMA and commit: the operands then sit in uniform registers, where
-    // these instructions take them from.  As the loop of a single lane the issuer needed about 600
-    // cycles per 64 of the reduction, whatever the tile ([16, 4096] x [4096, 4096]: 25 us).
-    const uint32_t one = lane == 0;
+    // The producer's and the issuer's loops run on a whole warp, uniform over it, and elect.sync picks
+    // the lane that issues the loads, MMAs and commits: these take their operands from uniform
+    // registers.  Under any other predicate (`lane == 0`) an MMA cost the issuing warp 68 cycles, so 21.
+    // What a stage costs that warp all the same, a wait (95), four MMAs (85) and the commit (130), is
+    // more than the MMAs of a 128 x 64 or 128 x 128 tile last: about 380 cycles per 64 of the reduction
+    // bound those shapes; the pair's 256 x 256 tile, 512 cycles of MMAs, hides it.  A second producer
+    // warp, or a look at the next stage's barrier ahead of the MMAs, gained nothing.
     const uint32_t full0 = smem_u32(&s->full[0]), empty0 = smem_u32(&s->empty[0]);
     const uint32_t a0 = smem_u32(&s->a[0][0]), b0 = smem_u32(&s->b[0][0]);
     if (warp == 0) {
@@ -431,21 +424,24 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             slice_range(w % p.slices, lo, hi);
             for (int kb = lo; kb < hi; ++kb) {
                 if (!(ok = wait_bar<CG>(empty0 + 8 * stage, phase ^ 1, s, 1, peer_abort))) break;
-                // the leader's barrier counts the bytes of both CTAs; parts out of range arrive as zeros
-                if (rank == 0) mbar_expect_tx_if(one, full0 + 8 * stage, CG * (C::A_STAGE + C::B_STAGE));
-                const uint32_t bar = lead_full0 + 8 * stage, at = a0 + stage * C::A_STAGE, bt = b0 + stage * C::B_STAGE;
-                if (p.a_mn) {
+                if (elect_one()) {
+                    // the leader's barrier counts the bytes of both CTAs; parts out of range arrive as zeros
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * stage, CG * (C::A_STAGE + C::B_STAGE));
+                    const uint32_t bar = lead_full0 + 8 * stage, at = a0 + stage * C::A_STAGE, bt = b0 + stage * C::B_STAGE;
+                    if (p.a_mn) {
 #pragma unroll
-                    for (int c = 0; c < BM / 64; ++c) tma_load_if<CG>(one, at + c * CHUNK, &map_a, bar, m0 + c * 64, kb * BK);
-                } else {
-                    tma_load_if<CG>(one, at, &map_a, bar, kb * BK, m0);
-                }
-                if (p.b_mn) {
+                        for (int c = 0; c < BM / 64; ++c) tma_load<CG>(at + c * CHUNK, &map_a, bar, m0 + c * 64, kb * BK);
+                    } else {
+                        tma_load<CG>(at, &map_a, bar, kb * BK, m0);
+                    }
+                    if (p.b_mn) {
 #pragma unroll
-                    for (int c = 0; c < C::BNC / 64; ++c) tma_load_if<CG>(one, bt + c * CHUNK, &map_b, bar, n0 + c * 64, kb * BK);
-                } else {
-                    tma_load_if<CG>(one, bt, &map_b, bar, kb * BK, n0);
+                        for (int c = 0; c < C::BNC / 64; ++c) tma_load<CG>(bt + c * CHUNK, &map_b, bar, n0 + c * 64, kb * BK);
+                    } else {
+                        tma_load<CG>(bt, &map_b, bar, kb * BK, n0);
+                    }
                 }
+                __syncwarp();
                 if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
             }
         }
@@ -481,14 +477,16 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     if (!(ok = wait_bar<CG>(full0 + 8 * stage, phase, s, 3, peer_abort))) break;
                     tc_fence_after();
                     const uint64_t adesc = adesc0 + stage * (C::A_STAGE >> 4), bdesc = bdesc0 + stage * (C::B_STAGE >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; ++k)
-                        umma_if<CG>(one, d, adesc + a_step * k, bdesc + b_step * k, idesc, (kb > lo || k) ? 1u : 0u);
-                    umma_commit_if<CG>(one, empty0 + 8 * stage);  // frees the slot (in both CTAs)
+                        for (int k = 0; k < BK / UMMA_K; ++k)
+                            umma<CG>(d, adesc + a_step * k, bdesc + b_step * k, idesc, (kb > lo || k) ? 1u : 0u);
+                        umma_commit<CG>(empty0 + 8 * stage);      // frees the slot (in both CTAs)
+                        if (kb == hi - 1) umma_commit<CG>(acc_full0 + 8 * buf);
+                    }
+                    __syncwarp();
                     if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
                 }
-                if (!ok) break;
-                umma_commit_if<CG>(one, acc_full0 + 8 * buf);
             }
         }
     } else {
@@ -499,18 +497,17 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         const int etid = threadIdx.x - 64;
         constexpr int PIECES = BN / 64;                           // 64-column pieces of a tile
         constexpr int MINE = PIECES >= 2 ? PIECES / 2 : 1;        // this warp's: half * MINE ...
-        const bool works = PIECES >= 2 || half == 0;
         uint8_t* const my_stage = &s->stage[ew][0][0];
         uint32_t full_phase[2] = {0, 0}, res_phase[2] = {0, 0};
         uint32_t seq = 0;                                         // pieces done: buffer seq & 1
         bool ok = true;
         // the residual of the piece at (row0, col0) into staging buffer b
         auto fetch_residual = [&](int row0, int col0, int b) {
-            mbar_expect_tx(&s->res[ew][b], PIECE);
-            tma_load<1>(my_stage + b * PIECE, &map_r, smem_u32(&s->res[ew][b]), col0, row0);
+            mbar_expect_tx(smem_u32(&s->res[ew][b]), PIECE);
+            tma_load<1>(smem_u32(my_stage + b * PIECE), &map_r, smem_u32(&s->res[ew][b]), col0, row0);
         };
         const bool ahead = p.has_res && p.tma_out && !DERIV;      // residual pieces fetched one ahead
-        if (ahead && works && lane == 0 && first < n_work) {
+        if (ahead && lane == 0 && first < n_work) {
             const int tile = first / p.slices;
             fetch_residual((tile / n_tiles) * C::TILE_M + (int)rank * BM + q * 32, (tile % n_tiles) * BN + half * MINE * 64, 0);
         }
@@ -536,117 +533,113 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             tc_fence_after();
             const uint32_t t_base = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * MINE * 64);
             const int rows = p.M - row0 < 32 ? p.M - row0 : 32;   // may be <= 0
-            if (works) {
 #pragma unroll 1
-                for (int i = 0; i < MINE; ++i) {
-                    const int col0 = n0 + (half * MINE + i) * 64;
-                    uint32_t r[64];
-                    tmem_ld32(t_base + (uint32_t)(i * 64), r);
-                    tmem_ld32(t_base + (uint32_t)(i * 64 + 32), r + 32);
-                    tmem_ld_wait();
-                    if (i == MINE - 1) {
-                        // the accumulator now lives in registers: hand the buffer back to the leader
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&s->acc_empty[buf]), 0));
-                    }
-                    if (p.out_f32) {
-                        // fp32 partial plane: two 32 x 32 pieces, one staging buffer each
-                        const int slice = w % p.slices;
-                        if (lane == 0) tma_wait_read<0>();
-                        __syncwarp();
-#pragma unroll
-                        for (int v = 0; v < 16; ++v)
-                            *reinterpret_cast<uint4*>(my_stage + (v >> 3) * PIECE + lane * 128 + (((v & 7) ^ (lane & 7)) << 4)) =
-                                make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
-                        fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0 && rows > 0) {
-                            if (col0 < p.N) tma_store_3d(&map_y, my_stage, col0, row0, slice);
-                            if (col0 + 32 < p.N) tma_store_3d(&map_y, my_stage + PIECE, col0 + 32, row0, slice);
-                            tma_commit();
-                        }
-                        continue;
-                    }
-                    // y (and the residual) in buffer b; the derivative in buffer 1 when there is one
-                    const int b = DERIV ? 0 : (int)(seq & 1);
-                    uint8_t* const yb = my_stage + b * PIECE;
-                    if (p.has_res) {
-                        if (p.tma_out) {
-                            if (!ahead && lane == 0) { tma_wait_read<0>(); fetch_residual(row0, col0, b); }
-                            ok = wait_bar_warp<CG>(&s->res[ew][b], res_phase[b], s, 7, peer_abort);
-                            res_phase[b] ^= 1;
-                        } else {
-                            piece_in(yb, static_cast<const unsigned short*>(p.res) + (int64_t)row0 * p.ld_res + col0, p.ld_res, rows, p.N - col0, lane);
-                            __syncwarp();
-                        }
-                    }
-                    const float* const bias = s->bias[buf] + (half * MINE + i) * 64;
-                    // r[8 v ..]: eight columns of z become four words of y and four of the derivative
-#pragma unroll
-                    for (int v = 0; v < 8; ++v) {
-                        const ulonglong2 b0 = *reinterpret_cast<const ulonglong2*>(bias + v * 8), b1 = *reinterpret_cast<const ulonglong2*>(bias + v * 8 + 4);
-                        const f32x2 bb[4] = {b0.x, b0.y, b1.x, b1.y};
-                        f32x2 y[4], d[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            activate2<KIND, DERIV>(add2_rn(pack2u(r[v * 8 + 2 * j], r[v * 8 + 2 * j + 1]), bb[j]), y[j], d[j]);
-                        if (p.has_res) {
-                            const uint4 rr = *reinterpret_cast<const uint4*>(yb + lane * 128 + ((v ^ (lane & 7)) << 4));
-                            const uint32_t h[4] = {rr.x, rr.y, rr.z, rr.w};
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) y[j] = add2_rn(y[j], widen_pair<DT>(h[j]));
-                        }
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            r[v * 8 + j] = narrow_pair<DT>(y[j]);
-                            if (DERIV) r[v * 8 + 4 + j] = narrow_pair<DT>(d[j]);
-                        }
-                    }
-                    // the stores that last read the buffers are done with them (a residual's own buffer was free before)
-                    if (p.tma_out && lane == 0) {
-                        if (DERIV) tma_wait_read<0>();
-                        else if (!p.has_res) tma_wait_read<1>();
-                    }
+            for (int i = 0; i < MINE; ++i) {
+                const int col0 = n0 + (half * MINE + i) * 64;
+                uint32_t r[64];
+                tmem_ld32(t_base + (uint32_t)(i * 64), r);
+                tmem_ld32(t_base + (uint32_t)(i * 64 + 32), r + 32);
+                tmem_ld_wait();
+                if (i == MINE - 1) {
+                    // the accumulator now lives in registers: hand the buffer back to the leader
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&s->acc_empty[buf]), 0));
+                }
+                if (p.out_f32) {
+                    // fp32 partial plane: two 32 x 32 pieces, one staging buffer each
+                    const int slice = w % p.slices;
+                    if (lane == 0) tma_wait_read<0>();
                     __syncwarp();
 #pragma unroll
-                    for (int v = 0; v < 8; ++v) {
-                        const int at = lane * 128 + ((v ^ (lane & 7)) << 4);
-                        *reinterpret_cast<uint4*>(yb + at) = make_uint4(r[v * 8], r[v * 8 + 1], r[v * 8 + 2], r[v * 8 + 3]);
-                        if (DERIV)
-                            *reinterpret_cast<uint4*>(my_stage + PIECE + at) = make_uint4(r[v * 8 + 4], r[v * 8 + 5], r[v * 8 + 6], r[v * 8 + 7]);
+                    for (int v = 0; v < 16; ++v)
+                        *reinterpret_cast<uint4*>(my_stage + (v >> 3) * PIECE + lane * 128 + (((v & 7) ^ (lane & 7)) << 4)) =
+                            make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0 && rows > 0) {
+                        if (col0 < p.N) tma_store_3d(&map_y, my_stage, col0, row0, slice);
+                        if (col0 + 32 < p.N) tma_store_3d(&map_y, my_stage + PIECE, col0 + 32, row0, slice);
+                        tma_commit();
                     }
-                    if (p.tma_out) {
-                        // the 32 x 64 piece leaves as one bulk tensor store, clipped at the tensor's edges
-                        fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (ok && rows > 0 && col0 < p.N) {
-                                tma_store_2d(&map_y, yb, col0, row0);
-                                if (DERIV) tma_store_2d(&map_d, my_stage + PIECE, col0, row0);
-                            }
-                            tma_commit();                         // also when nothing was stored: the groups count pieces
-                            if (ahead && i == MINE - 1 && ok && w + stride < n_work) {
-                                // the next tile's first residual goes into the other buffer once its store has read it
-                                const int nt = (w + stride) / p.slices;
-                                tma_wait_read<1>();
-                                fetch_residual((nt / n_tiles) * C::TILE_M + (int)rank * BM + q * 32,
-                                               (nt % n_tiles) * BN + half * MINE * 64, b ^ 1);
-                            }
-                        }
-                    } else {
-                        __syncwarp();
-                        if (ok && rows > 0 && col0 < p.N) {
-                            piece_out(yb, static_cast<unsigned short*>(p.y) + (int64_t)row0 * p.ld_y + col0, p.ld_y, rows, p.N - col0, lane);
-                            if (DERIV)
-                                piece_out(my_stage + PIECE, static_cast<unsigned short*>(p.d) + (int64_t)row0 * p.ld_d + col0, p.ld_d, rows, p.N - col0, lane);
-                        }
-                        __syncwarp();
-                    }
-                    ++seq;
+                    continue;
                 }
-            } else if (lane == 0) {
-                mbar_arrive_cluster(map_to_cta(smem_u32(&s->acc_empty[buf]), 0));
+                // y (and the residual) in buffer b; the derivative in buffer 1 when there is one
+                const int b = DERIV ? 0 : (int)(seq & 1);
+                uint8_t* const yb = my_stage + b * PIECE;
+                if (p.has_res) {
+                    if (p.tma_out) {
+                        if (!ahead && lane == 0) { tma_wait_read<0>(); fetch_residual(row0, col0, b); }
+                        ok = wait_bar_warp<CG>(&s->res[ew][b], res_phase[b], s, 7, peer_abort);
+                        res_phase[b] ^= 1;
+                    } else {
+                        piece_in(yb, static_cast<const unsigned short*>(p.res) + (int64_t)row0 * p.ld_res + col0, p.ld_res, rows, p.N - col0, lane);
+                        __syncwarp();
+                    }
+                }
+                const float* const bias = s->bias[buf] + (half * MINE + i) * 64;
+                // r[8 v ..]: eight columns of z become four words of y and four of the derivative
+#pragma unroll
+                for (int v = 0; v < 8; ++v) {
+                    const ulonglong2 b0 = *reinterpret_cast<const ulonglong2*>(bias + v * 8), b1 = *reinterpret_cast<const ulonglong2*>(bias + v * 8 + 4);
+                    const f32x2 bb[4] = {b0.x, b0.y, b1.x, b1.y};
+                    f32x2 y[4], d[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        activate2<KIND, DERIV>(add2_rn(pack2u(r[v * 8 + 2 * j], r[v * 8 + 2 * j + 1]), bb[j]), y[j], d[j]);
+                    if (p.has_res) {
+                        const uint4 rr = *reinterpret_cast<const uint4*>(yb + lane * 128 + ((v ^ (lane & 7)) << 4));
+                        const uint32_t h[4] = {rr.x, rr.y, rr.z, rr.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) y[j] = add2_rn(y[j], widen_pair<DT>(h[j]));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        r[v * 8 + j] = narrow_pair<DT>(y[j]);
+                        if (DERIV) r[v * 8 + 4 + j] = narrow_pair<DT>(d[j]);
+                    }
+                }
+                // the stores that last read the buffers are done with them (a residual's own buffer was free before)
+                if (p.tma_out && lane == 0) {
+                    if (DERIV) tma_wait_read<0>();
+                    else if (!p.has_res) tma_wait_read<1>();
+                }
+                __syncwarp();
+#pragma unroll
+                for (int v = 0; v < 8; ++v) {
+                    const int at = lane * 128 + ((v ^ (lane & 7)) << 4);
+                    *reinterpret_cast<uint4*>(yb + at) = make_uint4(r[v * 8], r[v * 8 + 1], r[v * 8 + 2], r[v * 8 + 3]);
+                    if (DERIV)
+                        *reinterpret_cast<uint4*>(my_stage + PIECE + at) = make_uint4(r[v * 8 + 4], r[v * 8 + 5], r[v * 8 + 6], r[v * 8 + 7]);
+                }
+                if (p.tma_out) {
+                    // the 32 x 64 piece leaves as one bulk tensor store, clipped at the tensor's edges
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (ok && rows > 0 && col0 < p.N) {
+                            tma_store_2d(&map_y, yb, col0, row0);
+                            if (DERIV) tma_store_2d(&map_d, my_stage + PIECE, col0, row0);
+                        }
+                        tma_commit();                         // also when nothing was stored: the groups count pieces
+                        if (ahead && i == MINE - 1 && ok && w + stride < n_work) {
+                            // the next tile's first residual goes into the other buffer once its store has read it
+                            const int nt = (w + stride) / p.slices;
+                            tma_wait_read<1>();
+                            fetch_residual((nt / n_tiles) * C::TILE_M + (int)rank * BM + q * 32,
+                                           (nt % n_tiles) * BN + half * MINE * 64, b ^ 1);
+                        }
+                    }
+                } else {
+                    __syncwarp();
+                    if (ok && rows > 0 && col0 < p.N) {
+                        piece_out(yb, static_cast<unsigned short*>(p.y) + (int64_t)row0 * p.ld_y + col0, p.ld_y, rows, p.N - col0, lane);
+                        if (DERIV)
+                            piece_out(my_stage + PIECE, static_cast<unsigned short*>(p.d) + (int64_t)row0 * p.ld_d + col0, p.ld_d, rows, p.N - col0, lane);
+                    }
+                    __syncwarp();
+                }
+                ++seq;
             }
         }
         if (lane == 0) tma_wait_read<0>();                        // the staging buffers are read before the CTA leaves
@@ -685,7 +678,7 @@ bool launch_one(const Maps& m, const Params& p, int grid, cudaStream_t st) {
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid, 1, 1);
-    cfg.blockDim = dim3(THREADS, 1, 1);
+    cfg.blockDim = dim3(Cfg<CG, BN>::THREADS, 1, 1);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];

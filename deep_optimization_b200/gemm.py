@@ -115,17 +115,17 @@ _DTYPE16 = {torch.bfloat16: _lib.ACT_DTYPE_BF16, torch.float16: _lib.ACT_DTYPE_F
 _DTYPES = {torch.float32: _lib.ACT_DTYPE_F32, **_DTYPE16}
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t as a matrix of its last dimension whose rows are contiguous and do not overlap."""
+def _rows(t: torch.Tensor):
+    """(t as a matrix of its last dimension whose rows are contiguous and do not overlap, its pitch)."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
-        t = t.contiguous()
-    return t
-
-
-def _pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, cols = t.shape
+    pitch, step = t.stride()
+    if (step != 1 and cols > 1) or (pitch < cols and rows > 1):
+        return t.contiguous(), cols
+    return t, pitch if rows > 1 else cols
 
 
 def linear_act_applies(x: torch.Tensor, weight: torch.Tensor) -> bool:
@@ -144,48 +144,53 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     the library's own choice."""
     if not x.is_cuda:
         raise RuntimeError("linear_act needs CUDA tensors: there is no CPU path")
-    dt = _DTYPE16.get(x.dtype)
-    if dt is None or weight.dtype != x.dtype:
-        raise TypeError(f"linear_act: x and weight must both be bfloat16 or both float16, got {x.dtype} and {weight.dtype}")
-    if activation not in _ACTIVATIONS:
+    dtype, dev = x.dtype, x.device
+    dt = _DTYPE16.get(dtype)
+    if dt is None or weight.dtype != dtype:
+        raise TypeError(f"linear_act: x and weight must both be bfloat16 or both float16, got {dtype} and {weight.dtype}")
+    kind = _ACTIVATIONS.get(activation)
+    if kind is None:
         raise ValueError(f"linear_act: activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
-    if derivative and activation in ("none", "relu"):
+    if derivative and kind in (_lib.ACT_KIND_NONE, _lib.ACT_KIND_RELU):
         raise ValueError("linear_act: the derivative is an output of the GELU and SiLU forms only")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.shape[1] == 0:
-        raise ValueError(f"linear_act: x [..., K] and weight [N, K] with K > 0, got {tuple(x.shape)} and {tuple(weight.shape)}")
-    N, K = weight.shape
-    shape = x.shape[:-1] + (N,)
-    bias_dt = 0
+    xs, ws = x.shape, weight.shape
+    if len(ws) != 2 or len(xs) < 1 or xs[-1] != ws[1] or ws[1] == 0:
+        raise ValueError(f"linear_act: x [..., K] and weight [N, K] with K > 0, got {tuple(xs)} and {tuple(ws)}")
+    N, K = ws
+    shape = (xs[0], N) if len(xs) == 2 else xs[:-1] + (N,)
+    bias_ptr, bias_dt = None, 0
     if bias is not None:
-        if bias.shape != (N,) or bias.dtype not in _DTYPES or bias.device != x.device:
+        bias_dt = _DTYPES.get(bias.dtype)
+        if bias_dt is None or bias.dim() != 1 or bias.shape[0] != N or bias.device != dev:
             raise ValueError("linear_act: bias must be [N], of a floating type of 16 or 32 bits, on x's device")
         bias = bias.contiguous()
-        bias_dt = _DTYPES[bias.dtype]
-    if weight.device != x.device:
+        bias_ptr = bias.data_ptr()
+    if weight.device != dev:
         raise ValueError("linear_act: weight must be on x's device")
-    x2, w2, r2 = _rows(x), _rows(weight), None
+    x2, ldx = _rows(x)
+    w2, ldw = _rows(weight)
+    M = x2.numel() // K
+    res_ptr, ldr = None, 0
     if residual is not None:
-        if residual.shape != shape or residual.dtype != x.dtype or residual.device != x.device:
+        if residual.shape != shape or residual.dtype != dtype or residual.device != dev:
             raise ValueError(f"linear_act: residual must have the result's shape {tuple(shape)}, type and device")
-        r2 = _rows(residual)
-    M = x2.shape[0]
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    d = torch.empty_like(y) if derivative else None
+        residual, ldr = _rows(residual)
+        res_ptr = residual.data_ptr()
+    y = x.new_empty(shape)
+    d = x.new_empty(shape) if derivative else None
     lib = _lib.load()
-    xp, wp, ldx, ldw = x2.data_ptr(), w2.data_ptr(), _pitch(x2), _pitch(w2)
-    ws_ptr = ws = None
-    need = 0
+    xp, wp = x2.data_ptr(), w2.data_ptr()
+    ws_ptr, need = None, 0
     if (xp | wp) & 15 or (ldx | ldw) & 7:                  # rows that may have to be copied first
         need = lib.act_linear_fwd_workspace(xp, ldx, wp, ldw, M, N, K, variant)
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        ws_ptr = ws.data_ptr()
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+            ws_ptr = workspace.data_ptr()
     with _lib.device_of(x):
-        rc = lib.act_linear_fwd(xp, ldx, wp, ldw, None if bias is None else bias.data_ptr(), bias_dt,
-                                None if r2 is None else r2.data_ptr(), 0 if r2 is None else _pitch(r2), dt, M, N, K,
-                                _ACTIVATIONS[activation], y.data_ptr(), N, None if d is None else d.data_ptr(), N, variant,
-                                ws_ptr, need, _lib.stream_ptr(x))
-    _lib.check(rc, "act_linear_fwd")
+        rc = lib.act_linear_fwd(xp, ldx, wp, ldw, bias_ptr, bias_dt, res_ptr, ldr, dt, M, N, K, kind, y.data_ptr(), N,
+                                None if d is None else d.data_ptr(), N, variant, ws_ptr, need, _lib.stream_ptr(x))
+    if rc:
+        _lib.check(rc, "act_linear_fwd")
     return (y, d) if derivative else y
 
 
@@ -243,16 +248,21 @@ def linear_backward(dz: torch.Tensor, x: Optional[torch.Tensor], weight: Optiona
     N = dz.shape[-1]
     K = weight.shape[1] if need_dx else x.shape[-1]
     M = dz.numel() // N if N else 0
-    dx = torch.empty(dz.shape[:-1] + (K,), dtype=dz.dtype, device=dz.device) if need_dx else None
+    dx = dz.new_empty(dz.shape[:-1] + (K,)) if need_dx else None
     dw = torch.empty((N, K), dtype=dw_dtype, device=dz.device) if need_dw else None
     if M == 0 or N == 0 or K == 0:                          # empty sums
         return (None if dx is None else dx.zero_()), (None if dw is None else dw.zero_())
-    g = _rows(dz)
-    x2 = None if x is None else _rows(x)
-    w2 = None if weight is None else _rows(weight)
+    g, ldg = _rows(dz)
+    xp = wp = None
+    ldx = ldw = 0
+    if need_dw:
+        x, ldx = _rows(x)
+        xp = x.data_ptr()
+    if need_dx:
+        weight, ldw = _rows(weight)
+        wp = weight.data_ptr()
     lib = _lib.load()
-    args = (g.data_ptr(), _pitch(g), None if x2 is None else x2.data_ptr(), 0 if x2 is None else _pitch(x2),
-            None if w2 is None else w2.data_ptr(), 0 if w2 is None else _pitch(w2))
+    args = (g.data_ptr(), ldg, xp, ldx, wp, ldw)
     with _lib.device_of(dz):
         need = lib.act_linear_bwd_workspace(*args, M, N, K, _DTYPES[dw_dtype], need_dx, need_dw, variant)
         ws = torch.empty(need, dtype=torch.uint8, device=dz.device) if need else None
