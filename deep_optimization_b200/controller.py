@@ -22,7 +22,7 @@ import torch.fx as FX
 from torch import nn
 from torch.fx.passes.shape_prop import ShapeProp
 
-from .layers import DOConv1d, DOConv2d, DOConv3d, DODepthPointConv2d, DOLinear, RMSNorm
+from .layers import DOConv1d, DOConv2d, DOConv3d, DODepthPointConv2d, DOLinear, DOLinearAct, RMSNorm
 from .modules.activations.act_layers import DODropout, DOGELU, DOMaxPool2d, DOReLU_Variance, DOSiLU
 from .modules.normalization.normalization_layers import DOBatchNorm2d, DOLayerNorm, DOSyncBatchNorm2d
 from .quantizer import Quantizer
@@ -304,6 +304,35 @@ class Controller:
             fused.append(new.target)
         return fused
 
+    def _fuse_linear_act(self, traced):
+        """A compressed linear layer whose only consumer is a compressed GELU or SiLU: the linear module
+        takes the activation over (DOLinearAct: the activation and the derivative it saves come out of the
+        product's epilogue) and the activation's node leaves the graph.  Parameters keep their names.
+        Returns the fused targets."""
+        fused = []
+        for node in list(traced.graph.nodes):
+            if node.op != "call_module" or len(node.users) != 1 or len(node.args) != 1 or node.kwargs:
+                continue
+            lin = traced.get_submodule(node.target)
+            if type(lin) is not DOLinear or self.meta[f"{node.target}"]["DIVISION"] is not None:
+                continue
+            user = next(iter(node.users))
+            if user.op != "call_module" or user.args != (node,) or user.kwargs:
+                continue
+            act = traced.get_submodule(user.target)
+            kind = {DOSiLU: "silu", DOGELU: "gelu" if getattr(act, "approximate", "") == "tanh" else "gelu_erf"}.get(type(act))
+            if kind is None or sum(n.op == "call_module" and n.target == node.target for n in traced.graph.nodes) != 1:
+                continue
+            new = DOLinearAct(lin.in_features, lin.out_features, kind, lin.bias is not None, clamp_alpha=self.layer_clamp,
+                              target_name=node.target, act_name=user.target, meta=self.meta)
+            new.weight, new.bias = lin.weight, lin.bias
+            parent_path, _, child = node.target.rpartition(".")
+            setattr(traced.get_submodule(parent_path), child, new)
+            user.replace_all_uses_with(node)
+            traced.graph.erase_node(user)
+            fused.append(node.target)
+        return fused
+
     @staticmethod
     def _fork_block_outputs(traced, targets):
         """A block output relu(batch_norm(x) + skip) usually feeds two consumers, the next block's
@@ -365,6 +394,7 @@ class Controller:
                     if type(mod) is nn.Dropout:
                         parent_path, _, child = name.rpartition(".")
                         setattr(traced.get_submodule(parent_path), child, DODropout(mod.p))
+            self.fused_linear_act = self._fuse_linear_act(traced) if self.config.get("fuse_linear_act", False) else []
             self.fused_add_layer_norm = []
             if self.config.get("fuse_add_layer_norm", True):
                 self.fused_add_layer_norm = self._fuse_add_layer_norm(traced)

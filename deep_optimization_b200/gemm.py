@@ -128,9 +128,10 @@ def _rows(t: torch.Tensor):
     return t, pitch if rows > 1 else cols
 
 
-def linear_act_applies(x: torch.Tensor, weight: torch.Tensor) -> bool:
-    """linear_act takes bf16 or fp16 CUDA tensors of one type and device, at least one input feature."""
-    return (x.is_cuda and x.dtype in _DTYPE16 and weight.dtype == x.dtype and weight.device == x.device
+def linear_act_applies(x: torch.Tensor, weight: torch.Tensor, cast_weight: bool = False) -> bool:
+    """linear_act takes bf16 or fp16 CUDA tensors of one type (`cast_weight`: the weight will be cast to x's)
+    and device, at least one input feature."""
+    return (x.is_cuda and x.dtype in _DTYPE16 and (cast_weight or weight.dtype == x.dtype) and weight.device == x.device
             and weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1] > 0)
 
 

@@ -14,7 +14,8 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from .modules.ops import GroupPACTClampFn, _DOConv1d, _DOConv2d, _DOConv3d, _DOLinear
+from .gemm import linear_act_applies
+from .modules.ops import GroupPACTClampFn, _DOConv1d, _DOConv2d, _DOConv3d, _DOLinear, _DOLinearAct
 
 
 class DOLinear(nn.Linear):
@@ -28,6 +29,45 @@ class DOLinear(nn.Linear):
             return _DOLinear.apply(x, self.weight, self.clamp_alpha, self.target_name, self.meta,
                                    self.ema_grad_meta, self.bias)
         return super().forward(x)
+
+
+_PLAIN_ACT = {"none": lambda z: z, "relu": F.relu, "gelu": lambda z: F.gelu(z, approximate="tanh"), "gelu_erf": F.gelu,
+              "silu": F.silu}
+
+
+class DOLinearAct(nn.Linear):
+    """A linear layer with its activation and, where given, a residual in one kernel:
+    `forward(x, residual=None)` = f(x W^T + b) + residual, f one of "none", "relu", "gelu" (tanh form),
+    "gelu_erf", "silu" (an extension: the reference has nn.Linear, the activation module and the addition).
+
+    Runs on `gemm.linear_act` when x is bf16 or fp16 on the GPU (under autocast: in its type, otherwise
+    when the weight has x's type), forward and backward, in training and evaluation; any other tensor
+    takes the three stock operators.  With `meta` (and in training) the layer's input is saved compressed
+    under `target_name` and the activation's derivative under `act_name`, as DOLinear and DOGELU / DOSiLU
+    save theirs."""
+
+    def __init__(self, in_features, out_features, activation="none", bias=True, clamp_alpha=3.0, target_name=None,
+                 act_name=None, meta=None):
+        super().__init__(in_features, out_features, bias)
+        if activation not in _PLAIN_ACT:
+            raise ValueError(f"DOLinearAct: activation must be one of {sorted(_PLAIN_ACT)}, got {activation!r}")
+        self.activation, self.clamp_alpha = activation, clamp_alpha
+        self.target_name, self.act_name, self.meta = target_name, act_name, meta
+
+    def forward(self, x, residual=None):
+        autocast = x.is_cuda and torch.is_autocast_enabled("cuda")
+        if autocast:
+            x = x.to(torch.get_autocast_dtype("cuda"))
+        if not linear_act_applies(x, self.weight, cast_weight=autocast):
+            y = _PLAIN_ACT[self.activation](F.linear(x, self.weight, self.bias))
+            return y if residual is None else y + residual
+        late = None                                          # a residual that the kernel does not take
+        if residual is not None and (residual.dtype != x.dtype or residual.device != x.device
+                                     or residual.shape != x.shape[:-1] + (self.out_features,)):
+            late, residual = residual, None
+        y = _DOLinearAct.apply(x, self.weight, self.bias, self.activation, residual, self.target_name, self.act_name,
+                               self.meta if self.training else None, self.clamp_alpha)
+        return y if late is None else y + late
 
 
 class _DOConvMixin:

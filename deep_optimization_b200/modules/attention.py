@@ -279,7 +279,7 @@ class RotaryAxes(nn.Module):
     def __init__(self, sections, base: float = 10000.0, interleaved: bool = False):
         super().__init__()
         self.sections, self.base, self.interleaved = tuple(int(n) for n in sections), float(base), bool(interleaved)
-        self.register_buffer("turns", rotary_turns(self.sections, self.base), persistent=False)
+        self.register_buffer("turns", rotary_turns(self.sections, self.base))
 
     def forward(self, qkv, heads, positions, kv_heads=None):
         return rotary_split_heads(qkv, heads, positions, self.turns, self.sections, kv_heads, self.interleaved)

@@ -15,10 +15,11 @@ import torch
 import torch.nn.functional as F
 from torch.amp import custom_bwd, custom_fwd
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 from torch.nn.modules.utils import _pair, _single, _triple
 
 from .. import codec
-from ..gemm import dw_from_packed
+from ..gemm import act_backward, dw_from_packed, linear_act, linear_backward
 from .module_utils import low_pass_upsampled, unified_dequantize, unified_quantize
 
 
@@ -256,6 +257,80 @@ class _DOLinear(Function):
             else:
                 db = dy2.sum(0, dtype=torch.float32).to(ctx.bias_dtype)
         return dx, dw, None, None, None, None, db
+
+
+class _DOLinearAct(Function):
+    """f(x W^T + b) + residual with the bias, the activation and the residual in the product's epilogue
+    (`gemm.linear_act`; an extension: the reference runs them as separate operators around F.linear,
+    Activation_Compression/modules/ops.py:438-479).  Backward needs x and, for GELU and SiLU, the
+    derivative f'(z), which the forward kernel returns; a ReLU's mask is the sign of its output, which is
+    kept (so a residual is added to it by a pass of its own when gradients are wanted).  With `meta` both are kept compressed, x as _DOLinear keeps it and the derivative as
+    _DOGELU / _DOSiLU keep theirs (`act_name` names its entry); without, as they are."""
+
+    @staticmethod
+    @custom_fwd(device_type="cuda")
+    def forward(ctx, input, weight, bias, activation, residual, target_name, act_name, meta, clamp_alpha):
+        ctx.needs = ctx.needs_input_grad
+        ctx.activation = activation
+        ctx.dtypes = (weight.dtype, None if bias is None else bias.dtype)
+        weight_compute = weight.to(input.dtype)
+        smooth = activation not in ("none", "relu")
+        wants_z = ctx.needs[0] or ctx.needs[1] or ctx.needs[2]
+        keep_sign = activation == "relu" and wants_z
+        out = linear_act(input, weight_compute, bias, activation, None if keep_sign else residual,
+                         derivative=smooth and wants_z)
+        y, d = out if smooth and wants_z else (out, None)
+        sign = y if keep_sign else None
+        if keep_sign and residual is not None:
+            y = y + residual
+        ctx.x_meta = ctx.d_meta = None
+        ctx.input_shape = input.shape
+        x_saved, d_saved = (input, None, None), (d, None, None)
+        if not ctx.needs[1]:
+            x_saved = (None, None, None)
+        elif meta is not None:
+            x_saved, ctx.x_meta, _ = unified_quantize(input, None, target_name, meta, clamp=True, clamp_alpha=clamp_alpha)
+        if d is not None and meta is not None:
+            d_saved, ctx.d_meta, _ = unified_quantize(d, None, act_name, meta, clamp=False, clamp_alpha=0.0)
+        ctx.save_for_backward(weight, *x_saved, *d_saved, sign)
+        return y
+
+    @staticmethod
+    @custom_bwd(device_type="cuda")
+    @once_differentiable
+    def backward(ctx, dy):
+        weight, x, x_scale, x_min, d, d_scale, d_min, sign = ctx.saved_tensors
+        need_dx, need_dw, need_db = ctx.needs[0], ctx.needs[1], ctx.needs[2]
+        dres = dy if ctx.needs[4] else None
+        if not (need_dx or need_dw or need_db):
+            return None, None, None, None, dres, None, None, None, None
+        if sign is not None:
+            d = (sign > 0).to(dy.dtype)
+        elif ctx.d_meta is not None:
+            d = unified_dequantize((d, d_scale, d_min), ctx.d_meta, None).to(dy.dtype)
+        if d is not None:
+            dz, db = act_backward(dy, d, bias_grad=need_db)
+        else:
+            dz = dy.contiguous()
+            db = dz.reshape(-1, dz.shape[-1])
+            db = None if not need_db else codec.col_sum(db) if codec.col_sum_applies(db) else db.sum(0, dtype=torch.float32)
+        wd, bd = ctx.dtypes
+        dz2 = dz.reshape(-1, dz.shape[-1])
+        dx = dw = None
+        if need_dw:
+            K = weight.shape[1]
+            if ctx.x_meta is None:
+                dw = linear_backward(dz, x, None, need_dx=False, dw_dtype=torch.float32 if wd == torch.float32 else None)[1]
+            elif FUSED_DW and x_scale is not None and x_scale.dtype == torch.float32 \
+                    and _fused_dw_applies(ctx.x_meta, None, dz2, K):
+                dw = dw_from_packed(dz2, x, x_scale, x_min, ctx.x_meta[0], ctx.x_meta[2], K)
+            else:
+                xq = unified_dequantize((x, x_scale, x_min), ctx.x_meta, None).to(dz.dtype).reshape(ctx.input_shape)
+                dw = linear_backward(dz, xq, None, need_dx=False, dw_dtype=torch.float32 if wd == torch.float32 else None)[1]
+            dw = dw.to(wd)
+        if need_dx:
+            dx = linear_backward(dz, None, weight.to(dz.dtype), need_dw=False)[0]
+        return dx, dw, None if db is None else db.to(bd), None, dres, None, None, None, None
 
 
 class GroupPACTClampFn(Function):
