@@ -870,8 +870,12 @@ def dropout_rng(device):
 
     Inside a CUDA graph capture the pair is an int64 [2] tensor on the device instead, taken from a
     stream that lives there, so that each replay draws a new mask; one call outside any capture has to
-    come first on each device."""
+    come first on each device.  A recomputation inside the capture draws a mask of its own: dropout under
+    `torch.utils.checkpoint` is for eager steps."""
     index = device.index if device.index is not None else torch.cuda.current_device()
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return dropout_rng(torch.device("cuda", index))
     if torch.cuda.is_current_stream_capturing():
         if index not in _graph_rng:
             raise RuntimeError("dropout_rng: run one step outside the capture first (the device's stream of mask "

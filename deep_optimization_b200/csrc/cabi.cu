@@ -57,7 +57,8 @@ extern "C" const char* act_strerror(int code) {
 
 // 2: hash and round-to-nearest modes are fixed-point (8 fraction bits, noise bytes); entry
 // points added for batch-norm statistics, BN+ReLU, backward constants and tiled addressing
-extern "C" int act_abi_version(void) { return 2; }
+// 3: entry points added for linear layers with an epilogue, dropout and rotary positions
+extern "C" int act_abi_version(void) { return 3; }
 
 // Greedy bit allocation.  Every layer i starts at b[i] bits and weighs w[i]; the
 // layer whose variance term C*(1/(2^b-1)^2 - 1/(2^(b-1)-1)^2) grows least loses

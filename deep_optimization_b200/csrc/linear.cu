@@ -376,6 +376,7 @@ bool is_16bit(int dtype) { return dtype == ACT_DTYPE_BF16 || dtype == ACT_DTYPE_
 bool tensor_ready(const void* p, int64_t ld) { return !((uintptr_t)p & 15) && !(ld & 7); }
 
 constexpr int kFewRows = 8;
+constexpr int kMostRows = 0x7FFFFC00;
 
 }  // namespace
 
@@ -392,6 +393,8 @@ extern "C" int act_linear_fwd(const void* x, int64_t ld_x, const void* w, int64_
                               void* workspace, size_t ws_bytes, void* stream)
 {
     if (!is_16bit(dtype) || (bias && !is_16bit(bias_dtype) && bias_dtype != ACT_DTYPE_F32)) return ACT_ERR_DTYPE;
+    // tile corners are 32-bit numbers
+    if (M > kMostRows || N > kMostRows || K > kMostRows) return ACT_ERR_SIZE;
     if (M < 0 || N < 0 || K < 1 || ld_x < K || ld_w < K || ld_y < N || (residual && ld_r < N) || (deriv && ld_d < N)) return ACT_ERR_SIZE;
     if (kind < ACT_KIND_NONE || kind > ACT_KIND_RELU || variant < 0 || variant > ACT_LINEAR_FEW_ROWS) return ACT_ERR_UNSUPPORTED;
     if (deriv && (kind == ACT_KIND_NONE || kind == ACT_KIND_RELU)) return ACT_ERR_UNSUPPORTED;
@@ -456,6 +459,7 @@ extern "C" int act_linear_bwd(const void* dz, int64_t ld_dz, const void* x, int6
                               void* workspace, size_t ws_bytes, void* stream)
 {
     if (!is_16bit(dtype) || (dw && dw_dtype != dtype && dw_dtype != ACT_DTYPE_F32)) return ACT_ERR_DTYPE;
+    if (M > kMostRows || N > kMostRows || K > kMostRows) return ACT_ERR_SIZE;
     if (M < 1 || N < 1 || K < 1 || ld_dz < N || (dw && (ld_x < K || ld_dw < K)) || (dx && (ld_w < K || ld_dx < K))) return ACT_ERR_SIZE;
     if (variant < 0 || variant > ACT_LINEAR_64) return ACT_ERR_UNSUPPORTED;
     if (!dx && !dw) return ACT_OK;

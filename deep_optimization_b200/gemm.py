@@ -128,6 +128,11 @@ def _rows(t: torch.Tensor):
     return t, pitch if rows > 1 else cols
 
 
+def _check_sizes(what: str, *sizes: int) -> None:
+    if max(sizes) > 0x7FFFFC00:
+        raise ValueError(f"{what}: at most {0x7FFFFC00} rows, features or columns, got {sizes}")
+
+
 def linear_act_applies(x: torch.Tensor, weight: torch.Tensor, cast_weight: bool = False) -> bool:
     """linear_act takes bf16 or fp16 CUDA tensors of one type (`cast_weight`: the weight will be cast to x's)
     and device, at least one input feature."""
@@ -171,6 +176,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     x2, ldx = _rows(x)
     w2, ldw = _rows(weight)
     M = x2.numel() // K
+    _check_sizes("linear_act", M, N, K)
     res_ptr, ldr = None, 0
     if residual is not None:
         if residual.shape != shape or residual.dtype != dtype or residual.device != dev:
@@ -208,18 +214,20 @@ def act_backward(dy: torch.Tensor, derivative: torch.Tensor, bias_grad: bool = T
     dy, derivative = dy.contiguous(), derivative.contiguous()
     N = dy.shape[-1]
     M = dy.numel() // N if N else 0
+    _check_sizes("act_backward", N)
     dz = torch.empty_like(dy)
     lib = _lib.load()
-    db = ws = None
+    db = db_ptr = ws_ptr = None
     need = 0
-    if bias_grad:
-        db = torch.empty(N, dtype=torch.float32, device=dy.device)
-        need = lib.act_mul_col_sum_workspace(M, N)
-        ws = torch.empty(need, dtype=torch.uint8, device=dy.device)
     with _lib.device_of(dy):
-        rc = lib.act_mul_col_sum(dy.data_ptr(), derivative.data_ptr(), _DTYPE16[dy.dtype], M, N, dz.data_ptr(),
-                                 None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), need,
-                                 _lib.stream_ptr(dy))
+        if bias_grad:
+            db = torch.empty(N, dtype=torch.float32, device=dy.device)
+            db_ptr = db.data_ptr()
+            need = lib.act_mul_col_sum_workspace(M, N)
+            workspace = torch.empty(need, dtype=torch.uint8, device=dy.device)
+            ws_ptr = workspace.data_ptr()
+        rc = lib.act_mul_col_sum(dy.data_ptr(), derivative.data_ptr(), _DTYPE16[dy.dtype], M, N, dz.data_ptr(), db_ptr, ws_ptr,
+                                 need, _lib.stream_ptr(dy))
     _lib.check(rc, "act_mul_col_sum")
     return dz, db
 
@@ -251,6 +259,7 @@ def linear_backward(dz: torch.Tensor, x: Optional[torch.Tensor], weight: Optiona
     M = dz.numel() // N if N else 0
     dx = dz.new_empty(dz.shape[:-1] + (K,)) if need_dx else None
     dw = torch.empty((N, K), dtype=dw_dtype, device=dz.device) if need_dw else None
+    _check_sizes("linear_backward", M, N, K)
     if M == 0 or N == 0 or K == 0:                          # empty sums
         return (None if dx is None else dx.zero_()), (None if dw is None else dw.zero_())
     g, ldg = _rows(dz)

@@ -273,3 +273,81 @@ def test_payload_defaults_are_unchanged(cuda_device):
     keys = set(_vit().state_dict())
     assert "pos_embed" in keys and not any("positions" in k or "turns" in k for k in keys)
     assert "pos_embed" not in set(_vit(rotary=True).state_dict())
+
+
+def test_refusals(cuda_device):
+    """Arguments that the host turns down before anything is launched."""
+    from deep_optimization_b200 import codec, gemm
+    from deep_optimization_b200.modules import attention
+    t = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device=cuda_device)
+    x, w = t(4, 16), t(8, 16)
+    for bad in (dict(x=t(4, 16, dt=torch.float32)), dict(w=t(8, 16, dt=torch.float16)), dict(w=t(8, 16, dt=torch.float32))):
+        with pytest.raises(TypeError):
+            gemm.linear_act(bad.get("x", x), bad.get("w", w))
+    for kw in (dict(activation="tanh"), dict(derivative=True), dict(activation="relu", derivative=True), dict(bias=t(9)),
+               dict(bias=t(8, dt=torch.int32)), dict(bias=torch.zeros(8)), dict(residual=t(4, 9)),
+               dict(residual=t(4, 8, dt=torch.float32)), dict(residual=t(8))):
+        with pytest.raises(ValueError):
+            gemm.linear_act(x, w, **kw)
+    for a, b in ((t(4, 15), w), (t(4, 0), t(8, 0)), (x, t(16)), (x, w.cpu())):
+        with pytest.raises(ValueError):
+            gemm.linear_act(a, b)
+    with pytest.raises(TypeError):
+        gemm.act_backward(x, t(4, 16, dt=torch.float16))
+    with pytest.raises(ValueError):
+        gemm.act_backward(x, t(4, 8))
+    with pytest.raises(TypeError):
+        gemm.linear_backward(t(4, 8, dt=torch.float32), x, w)
+    with pytest.raises(TypeError):
+        gemm.linear_backward(t(4, 8), x, w, dw_dtype=torch.float16)
+    for args in ((t(4, 9), x, w), (t(5, 8), x, w), (t(4, 8), t(4, 15), w), (t(4, 8), None, w), (t(4, 8), x, None)):
+        with pytest.raises(ValueError):
+            gemm.linear_backward(*args)
+    with pytest.raises(TypeError):
+        codec.dropout(t(4, dt=torch.int32), 0.5, (1, 1))
+    for kw in (dict(p=1.5), dict(residual=t(5)), dict(residual=t(4, dt=torch.float32)), dict(rng=t(2)), dict(rng=torch.zeros(2, dtype=torch.int64))):
+        with pytest.raises(ValueError):
+            codec.dropout(t(4), kw.get("p", 0.5), kw.get("rng", (1, 1)), kw.get("residual"))
+    turns = attention.rotary_turns((4, 4), device=cuda_device)
+    pos = t(5, 2, dt=torch.int64)
+    qkv = t(2, 5, 3 * 2 * 16)
+    ok = dict(qkv=qkv, heads=2, positions=pos, turns=turns, sections=(4, 4))
+    for kw in (dict(heads=5), dict(heads=0), dict(qkv=t(2, 96)), dict(positions=t(4, 2, dt=torch.int64)),
+               dict(positions=t(5, 1, dt=torch.int64)), dict(positions=t(3, 5, 2, dt=torch.int64)), dict(turns=turns[:7]),
+               dict(turns=turns.int()), dict(turns=turns.cpu()), dict(sections=(4, 5)), dict(sections=(4, 4, 0, 0, 0)),
+               dict(sections=(-1, 9)), dict(sections=())):
+        with pytest.raises(ValueError):
+            attention.rotary_split(**{**ok, **kw})
+    for kw in (dict(positions=pos.float()), dict(positions=pos.cpu()), dict(qkv=qkv.double())):
+        with pytest.raises(TypeError):
+            attention.rotary_split(**{**ok, **kw})
+    g = t(2, 2, 5, 16)
+    for dk, dv in ((t(2, 2, 4, 16), g), (g, t(2, 1, 5, 16)), (g, t(2, 2, 5, 16, dt=torch.float16))):
+        with pytest.raises(ValueError):
+            attention.rotary_merge(g, dk, dv, pos, turns, (4, 4))
+    with pytest.raises(ValueError):
+        attention.rotary_heads(t(5, 16), pos, turns, (4, 4))
+
+
+def test_two_streams_at_once(cuda_device):
+    """Calls in flight on two streams share nothing: each result is that of its own call."""
+    from deep_optimization_b200 import gemm
+    torch.manual_seed(8)
+    pairs = [(torch.randn(1003, 771, device=cuda_device).bfloat16(), torch.randn(997, 771, device=cuda_device).bfloat16()) for _ in range(2)]
+    want = []
+    for x, w in pairs:
+        y, d = gemm.linear_act(x, w, activation="gelu", derivative=True)
+        dz, db = gemm.act_backward(y, d)
+        want.append((y, d, dz, db, *gemm.linear_backward(dz, x, w)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for _ in range(3):
+        for i, (x, w) in enumerate(pairs):
+            with torch.cuda.stream(streams[i]):
+                y, d = gemm.linear_act(x, w, activation="gelu", derivative=True)
+                dz, db = gemm.act_backward(y, d)
+                got[i] = (y, d, dz, db, *gemm.linear_backward(dz, x, w))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))

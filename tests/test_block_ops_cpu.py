@@ -50,6 +50,7 @@ def test_linear_forward_refusals(lib):
     assert _fwd(lib, kind=0, d=P, ldd=64) == UNSUPPORTED and _fwd(lib, kind=4, d=P, ldd=64) == UNSUPPORTED
     assert _fwd(lib, x=None) == NULL and _fwd(lib, w=None) == NULL and _fwd(lib, y=None) == NULL
     assert _fwd(lib, x=ODD) == ALIGN and _fwd(lib, bias=ctypes.c_void_p(4098), bias_dt=0) == ALIGN
+    assert _fwd(lib, M=0x7FFFFC01) == SIZE and _fwd(lib, N=0x7FFFFFFF, ldy=1 << 31) == SIZE
     assert _fwd(lib, M=0) == 0 and _fwd(lib, N=0, ldy=0) == 0
     # rows that a bulk copy cannot read need the workspace
     need = lib.act_linear_fwd_workspace(P, 65, P, 64, 32, 64, 64, 0)
@@ -70,6 +71,7 @@ def test_linear_backward_refusals(lib):
     assert _bwd(lib, M=0) == SIZE and _bwd(lib, N=0) == SIZE and _bwd(lib, K=0) == SIZE
     assert _bwd(lib, lddz=63) == SIZE and _bwd(lib, ldx=63) == SIZE and _bwd(lib, ldw=63) == SIZE
     assert _bwd(lib, lddx=63) == SIZE and _bwd(lib, lddw=63) == SIZE
+    assert _bwd(lib, M=0x7FFFFC01) == SIZE
     assert _bwd(lib, variant=4) == UNSUPPORTED
     assert _bwd(lib, dx=None, dw=None) == 0
     assert _bwd(lib, dz=None) == NULL and _bwd(lib, w=None) == NULL and _bwd(lib, x=None) == NULL
@@ -174,3 +176,12 @@ def test_turns_are_the_frequencies():
     for got, f in zip(t, (1.0, 100.0 ** (-1 / 3), 100.0 ** (-2 / 3), 1.0, 0.1)):
         # three roundings of 2^-53 relative, then half a unit
         assert abs(Fraction(got) - Fraction(f / (2 * math.pi)) * 2 ** 64) <= Fraction(f) * 2 ** 12
+
+
+def test_dropout_in_a_capture_needs_a_step_outside_first(monkeypatch):
+    from deep_optimization_b200 import codec
+    monkeypatch.setattr(codec, "_graph_rng", {})
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="outside the capture"):
+        codec.dropout_rng(torch.device("cuda", 0))
