@@ -242,7 +242,7 @@ __device__ __forceinline__ f32x2 rcp_approx2(f32x2 v) {
 __device__ __forceinline__ f32x2 both(float v) { return pack2(v, v); }
 
 // f(z) and f'(z) of two values, on packed fp32 pairs: as single operations the GELU with its derivative
-// took more issue slots per tile than K = 768 of MMAs last (bf16 50432 x 768 x 2304: 192 us, now 155).
+// took more issue slots per tile than K = 768 of MMAs last (bf16 50432 x 768 x 2304: 192 us, 171 on pairs).
 // The exponential and reciprocal instructions are within 2^-22, which a 16-bit result does not show.
 //
 // GELU in its tanh form is z times the logistic function s of 2u, u = k (z + c z^3).  z^2 is held to
@@ -577,8 +577,14 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         __syncwarp();
                     }
                 }
+                // the stores that last read the buffers must be done with them: waited for here when there
+                // are two outputs, whose words would else fill the registers (GELU with derivative, K = 768:
+                // 182 us after the arithmetic, 174 before it), and after the arithmetic when there is one
+                if (DERIV) {
+                    if (p.tma_out && lane == 0) tma_wait_read<0>();
+                    __syncwarp();
+                }
                 const float* const bias = s->bias[buf] + (half * MINE + i) * 64;
-                // r[8 v ..]: eight columns of z become four words of y and four of the derivative
 #pragma unroll
                 for (int v = 0; v < 8; ++v) {
                     const ulonglong2 b0 = *reinterpret_cast<const ulonglong2*>(bias + v * 8), b1 = *reinterpret_cast<const ulonglong2*>(bias + v * 8 + 4);
@@ -593,24 +599,22 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 #pragma unroll
                         for (int j = 0; j < 4; ++j) y[j] = add2_rn(y[j], widen_pair<DT>(h[j]));
                     }
+                    const int at = lane * 128 + ((v ^ (lane & 7)) << 4);
+                    if (DERIV) {
+                        *reinterpret_cast<uint4*>(yb + at) = make_uint4(narrow_pair<DT>(y[0]), narrow_pair<DT>(y[1]), narrow_pair<DT>(y[2]), narrow_pair<DT>(y[3]));
+                        *reinterpret_cast<uint4*>(my_stage + PIECE + at) =
+                            make_uint4(narrow_pair<DT>(d[0]), narrow_pair<DT>(d[1]), narrow_pair<DT>(d[2]), narrow_pair<DT>(d[3]));
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        r[v * 8 + j] = narrow_pair<DT>(y[j]);
-                        if (DERIV) r[v * 8 + 4 + j] = narrow_pair<DT>(d[j]);
+                        for (int j = 0; j < 4; ++j) r[v * 8 + j] = narrow_pair<DT>(y[j]);   // eight columns of z become four words
                     }
                 }
-                // the stores that last read the buffers are done with them (a residual's own buffer was free before)
-                if (p.tma_out && lane == 0) {
-                    if (DERIV) tma_wait_read<0>();
-                    else if (!p.has_res) tma_wait_read<1>();
-                }
-                __syncwarp();
+                if (!DERIV) {
+                    if (p.tma_out && lane == 0 && !p.has_res) tma_wait_read<1>();    // a residual's own buffer was free before
+                    __syncwarp();
 #pragma unroll
-                for (int v = 0; v < 8; ++v) {
-                    const int at = lane * 128 + ((v ^ (lane & 7)) << 4);
-                    *reinterpret_cast<uint4*>(yb + at) = make_uint4(r[v * 8], r[v * 8 + 1], r[v * 8 + 2], r[v * 8 + 3]);
-                    if (DERIV)
-                        *reinterpret_cast<uint4*>(my_stage + PIECE + at) = make_uint4(r[v * 8 + 4], r[v * 8 + 5], r[v * 8 + 6], r[v * 8 + 7]);
+                    for (int v = 0; v < 8; ++v)
+                        *reinterpret_cast<uint4*>(yb + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(r[v * 8], r[v * 8 + 1], r[v * 8 + 2], r[v * 8 + 3]);
                 }
                 if (p.tma_out) {
                     // the 32 x 64 piece leaves as one bulk tensor store, clipped at the tensor's edges
