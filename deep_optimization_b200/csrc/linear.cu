@@ -14,63 +14,88 @@ int stream_grid_for(int64_t n_blocks_wanted, int blocks_per_sm, int waves = 1); 
 
 namespace linear {
 
-// ------------------------------------------------------------------ few rows: one warp per column
-// For up to eight rows of x the product reads W once and does next to nothing else: bound by HBM (or,
-// when W is small, by the launch).  A warp computes column n of all rows: its lanes take 16-byte
-// pieces of the row W[n, :] (two bytes where rows are not aligned), x comes out of L1, the sums are
-// joined by shuffles and lane m finishes row m.  [1, 768] x [768, 2304]: 3.0 us.
-template <int MB, bool VEC>
-__global__ void __launch_bounds__(256)
+// ------------------------------------------------------------------ few rows: warps per column
+// For a few rows of x the product reads W once and does next to nothing else: bound by HBM (or,
+// when W is small, by the launch).  Warps walk rows of W (COLS of them each, so that x is widened once
+// for both) in 16-byte pieces, two bytes where rows are not aligned, several pieces in flight; x comes
+// out of L1.  Where there are few columns, KS warps share each column's reduction and join their sums
+// through shared memory in a fixed order.  KS is chosen so that the GPU has work for about sixteen
+// warps per SM ([1, 4096] x [4096, 1024]: 10.2 us with one warp per column, 4.5 so).  One row of 768 against
+// 2304 columns takes 2.9 us, against [4096, 4096] out of HBM 9.2 us (33.6 MB, floor 5.1).
+constexpr int kFewWarps = 8;
+
+template <int DT, int MB, int COLS, bool VEC>
+__global__ void __launch_bounds__(kFewWarps * 32)
 few_rows_kernel(const unsigned short* __restrict__ x, int64_t ld_x, const unsigned short* __restrict__ w, int64_t ld_w,
                 const void* __restrict__ bias, int bias_dtype, const unsigned short* __restrict__ res, int64_t ld_res,
-                int M, int N, int K, int kind, int dtype, unsigned short* __restrict__ y, int64_t ld_y,
+                int M, int N, int K, int ks_count, int kind, unsigned short* __restrict__ y, int64_t ld_y,
                 unsigned short* __restrict__ d, int64_t ld_d)
 {
-    const int lane = threadIdx.x & 31;
-    const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (n >= N) return;
-    const unsigned short* wr = w + (int64_t)n * ld_w;
-    float acc[MB];
+    constexpr int V = VEC ? 8 : 1, U = COLS == 1 ? 4 : 2;     // elements per access, accesses in flight per column
+    __shared__ float part[kFewWarps][COLS * MB];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int ks = warp % ks_count, group = warp / ks_count, groups = kFewWarps / ks_count;
+    const int64_t n0 = ((int64_t)blockIdx.x * groups + group) * COLS;
+    float acc[COLS][MB];
 #pragma unroll
-    for (int m = 0; m < MB; ++m) acc[m] = 0.0f;
-    if (VEC) {
-#pragma unroll 4
-        for (int k = lane * 8; k < K; k += 256) {             // K is a multiple of 8
-            const uint4 wv = ldg_stream_v4(wr + k);
-            const uint32_t wu[4] = {wv.x, wv.y, wv.z, wv.w};
-            float wf[8];
+    for (int c = 0; c < COLS; ++c)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { wf[2 * i] = widen16(wu[i] & 0xFFFFu, dtype); wf[2 * i + 1] = widen16(wu[i] >> 16, dtype); }
+        for (int m = 0; m < MB; ++m) acc[c][m] = 0.0f;
+    const int64_t step = (int64_t)ks_count * 32 * V;
+    for (int64_t k = ((int64_t)ks * 32 + lane) * V; k < K && n0 < N; k += U * step) {     // VEC: K is a multiple of 8
+        uint4 wv[U][COLS];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) {
+                wv[u][c] = make_uint4(0u, 0u, 0u, 0u);
+                if (k + u * step < K && n0 + c < N) {
+                    const unsigned short* at = w + (n0 + c) * ld_w + k + u * step;
+                    if (VEC) wv[u][c] = ldg_stream_v4(at);
+                    else wv[u][c].x = __ldg(at);
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k + u * step >= K) break;
 #pragma unroll
             for (int m = 0; m < MB; ++m) {
                 if (m >= M) continue;
-                const uint4 xv = ldg_nc_v4(x + m * ld_x + k);
+                uint4 xv = make_uint4(0u, 0u, 0u, 0u);
+                if (VEC) xv = ldg_nc_v4(x + m * ld_x + k + u * step);
+                else xv.x = __ldg(x + m * ld_x + k + u * step);
                 const uint32_t xu[4] = {xv.x, xv.y, xv.z, xv.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    acc[m] = __fmaf_rn(widen16(xu[i] & 0xFFFFu, dtype), wf[2 * i], acc[m]);
-                    acc[m] = __fmaf_rn(widen16(xu[i] >> 16, dtype), wf[2 * i + 1], acc[m]);
+                for (int c = 0; c < COLS; ++c) {
+                    const uint32_t wu[4] = {wv[u][c].x, wv[u][c].y, wv[u][c].z, wv[u][c].w};
+#pragma unroll
+                    for (int i = 0; i < (VEC ? 4 : 1); ++i) {
+                        acc[c][m] = __fmaf_rn(widen_lo<DT>(xu[i]), widen_lo<DT>(wu[i]), acc[c][m]);
+                        if (VEC) acc[c][m] = __fmaf_rn(widen_hi<DT>(xu[i]), widen_hi<DT>(wu[i]), acc[c][m]);
+                    }
                 }
             }
         }
-    } else {
-#pragma unroll 4
-        for (int k = lane; k < K; k += 32) {
-            const float wf = widen16(__ldg(wr + k), dtype);
+    }
 #pragma unroll
-            for (int m = 0; m < MB; ++m)
-                if (m < M) acc[m] = __fmaf_rn(widen16(__ldg(x + m * ld_x + k), dtype), wf, acc[m]);
+    for (int c = 0; c < COLS; ++c)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            float a = acc[c][m];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) a = __fadd_rn(a, __shfl_xor_sync(0xffffffffu, a, o));
+            if (lane == 0) part[warp][c * MB + m] = a;
         }
-    }
-    float mine = 0.0f;
-#pragma unroll
-    for (int m = 0; m < MB; ++m) {
-#pragma unroll
-        for (int o = 16; o; o >>= 1) acc[m] = __fadd_rn(acc[m], __shfl_xor_sync(0xffffffffu, acc[m], o));
-        if (lane == m) mine = acc[m];
-    }
-    if (lane >= M) return;
-    const float z = __fadd_rn(mine, bias ? load_any(bias, n, bias_dtype) : 0.0f);
+    __syncthreads();
+    // one thread per output of the block
+    const int t = threadIdx.x;
+    if (t >= groups * COLS * MB) return;
+    const int g = t / (COLS * MB), cm = t - g * (COLS * MB), c = cm / MB, m = cm - c * MB;
+    const int64_t n = ((int64_t)blockIdx.x * groups + g) * COLS + c;
+    if (m >= M || n >= N) return;
+    float z = part[g * ks_count][cm];
+    for (int i = 1; i < ks_count; ++i) z = __fadd_rn(z, part[g * ks_count + i][cm]);
+    if (bias) z = __fadd_rn(z, load_any(bias, n, bias_dtype));
     float yv = z, dv = 0.0f;
     switch (kind) {
         case ACT_KIND_RELU: activate<ACT_KIND_RELU, false>(z, yv, dv); break;
@@ -79,9 +104,34 @@ few_rows_kernel(const unsigned short* __restrict__ x, int64_t ld_x, const unsign
         case ACT_KIND_GELU_ERF: activate<ACT_KIND_GELU_ERF, true>(z, yv, dv); break;
         default: break;
     }
-    if (res) yv = __fadd_rn(yv, widen16(res[lane * ld_res + n], dtype));
-    y[lane * ld_y + n] = (unsigned short)round_pair(yv, 0.0f, dtype);
-    if (d) d[lane * ld_d + n] = (unsigned short)round_pair(dv, 0.0f, dtype);
+    if (res) yv = __fadd_rn(yv, widen_lo<DT>(res[m * ld_res + n]));
+    y[m * ld_y + n] = (unsigned short)round_pair(yv, 0.0f, DT);
+    if (d) d[m * ld_d + n] = (unsigned short)round_pair(dv, 0.0f, DT);
+}
+
+struct FewArgs {
+    const unsigned short *x, *w, *res;
+    const void* bias;
+    unsigned short *y, *d;
+    int64_t ld_x, ld_w, ld_r, ld_y, ld_d;
+    int bias_dtype, M, N, K, kind;
+};
+template <int DT, int MB, int COLS>
+void few_rows(const FewArgs& a, bool vec, int sms, cudaStream_t st) {
+    const int64_t units = ((int64_t)a.N + COLS - 1) / COLS;
+    int ks = 1;
+    while (ks < kFewWarps && units * ks < (int64_t)sms * 16 && (int64_t)a.K > (int64_t)ks * 512) ks *= 2;
+    const int64_t grid = (units * ks + kFewWarps - 1) / kFewWarps;
+    if (vec) few_rows_kernel<DT, MB, COLS, true><<<(unsigned)grid, kFewWarps * 32, 0, st>>>(a.x, a.ld_x, a.w, a.ld_w, a.bias, a.bias_dtype,
+                 a.res, a.ld_r, a.M, a.N, a.K, ks, a.kind, a.y, a.ld_y, a.d, a.ld_d);
+    else few_rows_kernel<DT, MB, COLS, false><<<(unsigned)grid, kFewWarps * 32, 0, st>>>(a.x, a.ld_x, a.w, a.ld_w, a.bias, a.bias_dtype,
+                 a.res, a.ld_r, a.M, a.N, a.K, ks, a.kind, a.y, a.ld_y, a.d, a.ld_d);
+}
+template <int DT> void few_rows_any(const FewArgs& a, bool vec, int sms, cudaStream_t st) {
+    if (a.M == 1) few_rows<DT, 1, 1>(a, vec, sms, st);
+    else if (a.M == 2) few_rows<DT, 2, 2>(a, vec, sms, st);
+    else if (a.M <= 4) few_rows<DT, 4, 2>(a, vec, sms, st);
+    else few_rows<DT, 8, 2>(a, vec, sms, st);
 }
 
 // Rows of 16-bit elements copied to a pitch that a bulk tensor copy can read (a multiple of 16 bytes):
@@ -377,6 +427,14 @@ bool is_16bit(int dtype) { return dtype == ACT_DTYPE_BF16 || dtype == ACT_DTYPE_
 bool tensor_ready(const void* p, int64_t ld) { return !((uintptr_t)p & 15) && !(ld & 7); }
 
 constexpr int kFewRows = 8;
+// Warps per column or tensor-core tiles.  Measured, columns / 128 x 64 tiles, us: one row [768 -> 768] 2.5 / 5.4,
+// [4096 -> 1024] 4.5 / 16, [4096 -> 4096] 9.2 / 22; four rows 4.0 / 5.4, 6.1 / 16, 15 / 22; eight rows 6.2 / 5.4,
+// 9.0 / 16, 24 / 22.  Above four rows only a reduction longer than the row of outputs, which leaves few
+// tiles with much to do each, is better served by columns.
+bool use_columns(int M, int N, int K, int variant) {
+    if (variant) return variant == ACT_LINEAR_FEW_ROWS;
+    return M <= 4 || (M <= kFewRows && K > N);
+}
 constexpr int kMostRows = 0x7FFFFC00;
 
 }  // namespace
@@ -384,7 +442,7 @@ constexpr int kMostRows = 0x7FFFFC00;
 extern "C" size_t act_linear_fwd_workspace(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int M, int N, int K, int variant)
 {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    if (variant == ACT_LINEAR_FEW_ROWS || (variant == 0 && M <= kFewRows)) return 0;
+    if (use_columns(M, N, K, variant)) return 0;
     return pad_bytes(Mat{x, ld_x, M, K}) + pad_bytes(Mat{w, ld_w, N, K});
 }
 
@@ -405,22 +463,14 @@ extern "C" int act_linear_fwd(const void* x, int64_t ld_x, const void* w, int64_
     if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)residual | (uintptr_t)deriv) & 1) return ACT_ERR_ALIGN;
     if (bias && ((uintptr_t)bias & (bias_dtype == ACT_DTYPE_F32 ? 3 : 1))) return ACT_ERR_ALIGN;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (variant == ACT_LINEAR_FEW_ROWS || (variant == 0 && M <= kFewRows)) {
-        const auto* xp = static_cast<const unsigned short*>(x);
-        const auto* wp = static_cast<const unsigned short*>(w);
-        const auto* rp = static_cast<const unsigned short*>(residual);
-        auto* yp = static_cast<unsigned short*>(y);
-        auto* dp = static_cast<unsigned short*>(deriv);
+    if (use_columns(M, N, K, variant)) {
+        const FewArgs f = {static_cast<const unsigned short*>(x), static_cast<const unsigned short*>(w),
+                           static_cast<const unsigned short*>(residual), bias, static_cast<unsigned short*>(y),
+                           static_cast<unsigned short*>(deriv), ld_x, ld_w, ld_r, ld_y, ld_d, bias_dtype, M, N, K, kind};
         const bool vec = !((K | ld_x | ld_w) & 7) && !(((uintptr_t)x | (uintptr_t)w) & 15);
-        const int grid = (int)ceil_div(N, 8);
-#define ACT_FEW(MB)                                                                                                          \
-    (vec ? few_rows_kernel<MB, true><<<grid, 256, 0, st>>>(xp, ld_x, wp, ld_w, bias, bias_dtype, rp, ld_r, M, N, K, kind, dtype, yp, ld_y, dp, ld_d) \
-         : few_rows_kernel<MB, false><<<grid, 256, 0, st>>>(xp, ld_x, wp, ld_w, bias, bias_dtype, rp, ld_r, M, N, K, kind, dtype, yp, ld_y, dp, ld_d))
-        if (M == 1) ACT_FEW(1);
-        else if (M == 2) ACT_FEW(2);
-        else if (M <= 4) ACT_FEW(4);
-        else ACT_FEW(8);
-#undef ACT_FEW
+        const int sms = act::stream_grid_for((int64_t)1 << 40, 1, 1);
+        if (dtype == ACT_DTYPE_BF16) few_rows_any<ACT_DTYPE_BF16>(f, vec, sms, st);
+        else few_rows_any<ACT_DTYPE_F16>(f, vec, sms, st);
         return cudaGetLastError() == cudaSuccess ? ACT_OK : ACT_ERR_LAUNCH;
     }
     Mat a = {x, ld_x, M, K}, b = {w, ld_w, N, K};

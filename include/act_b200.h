@@ -52,7 +52,7 @@ extern "C" {
 #define ACT_LINEAR_PAIR 1          /* CTA pairs on 256 x 256 tiles */
 #define ACT_LINEAR_128 2           /* one CTA per 128 x 128 tile */
 #define ACT_LINEAR_64 3            /* one CTA per 128 x 64 tile */
-#define ACT_LINEAR_FEW_ROWS 4      /* forward, up to eight rows: a warp per column, no tensor cores */
+#define ACT_LINEAR_FEW_ROWS 4      /* forward, up to eight rows: warps per column, no tensor cores */
 
 /* flags of act_fp8_gemm */
 #define ACT_GEMM_B_IS_NK 1         /* B is stored [N,K] (K contiguous, like nn.Linear weights)        */

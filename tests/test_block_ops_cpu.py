@@ -58,7 +58,7 @@ def test_linear_forward_refusals(lib):
     assert _fwd(lib, ldx=65) == WORKSPACE and _fwd(lib, ldx=65, ws=P, ws_bytes=need - 1) == WORKSPACE
     assert _fwd(lib, ldx=65, ws=ctypes.c_void_p(4104), ws_bytes=need) == ALIGN
     assert lib.act_linear_fwd_workspace(P, 64, P, 64, 32, 64, 64, 0) == 0
-    assert lib.act_linear_fwd_workspace(P, 65, P, 64, 8, 64, 64, 0) == 0        # few rows read in place
+    assert lib.act_linear_fwd_workspace(P, 65, P, 64, 4, 64, 64, 0) == 0        # few rows read in place
 
 
 def _bwd(lib, dz=P, lddz=64, x=P, ldx=64, w=P, ldw=64, dt=1, M=32, N=64, K=64, dx=P, lddx=64, dw=P, lddw=64, dwt=1, variant=0,

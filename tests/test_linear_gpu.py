@@ -83,10 +83,12 @@ def test_forward(cuda_device, dtype, act, variant, shape):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 8])
-@pytest.mark.parametrize("shape", [(768, 768), (1, 1), (33, 7), (100, 264), (2304, 776)])
+@pytest.mark.parametrize("shape", [(768, 768), (1, 1), (33, 7), (100, 264), (2304, 776), (5, 4096), (130, 4099), (3, 1025)])
 def test_few_rows(cuda_device, dtype, M, shape):
     for i, act in enumerate(ACTS):
-        _linear_case(M, *shape, dtype, act, i % 2 == 0, ("", "16", "32")[i % 3], act not in ("none", "relu"), 0, cuda_device, seed=M + i)
+        for variant in (0, 4):
+            _linear_case(M, *shape, dtype, act, i % 2 == 0, ("", "16", "32")[i % 3], act not in ("none", "relu"), variant,
+                         cuda_device, seed=M + i)
 
 
 @pytest.mark.parametrize("variant", VARIANTS)
