@@ -56,7 +56,7 @@ template <int CG, int BN> struct __align__(1024) Smem {
     uint8_t a[Cfg<CG, BN>::STAGES][Cfg<CG, BN>::A_STAGE];
     uint8_t b[Cfg<CG, BN>::STAGES][Cfg<CG, BN>::B_STAGE];
     uint8_t stage[Cfg<CG, BN>::EPI_WARPS][2][PIECE];          // 128-byte rows, 16-byte pieces xor-swizzled by row & 7
-    float bias[2][BN];
+    float bias[Cfg<CG, BN>::EPI_WARPS][64];       // of the piece a warp works on
     uint64_t full[Cfg<CG, BN>::STAGES], empty[Cfg<CG, BN>::STAGES], acc_full[2], acc_empty[2], res[Cfg<CG, BN>::EPI_WARPS][2];
     uint32_t tmem_base;
     volatile uint32_t abort;
@@ -494,7 +494,6 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         const int ew = warp - 2;
         const int q = warp & 3;                                   // TMEM lane quarter this warp may read
         const int half = ew >> 2;                                 // which half of the tile's pieces
-        const int etid = threadIdx.x - 64;
         constexpr int PIECES = BN / 64;                           // 64-column pieces of a tile
         constexpr int MINE = PIECES >= 2 ? PIECES / 2 : 1;        // this warp's: half * MINE ...
         uint8_t* const my_stage = &s->stage[ew][0][0];
@@ -512,23 +511,27 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             fetch_residual((tile / n_tiles) * C::TILE_M + (int)rank * BM + q * 32, (tile % n_tiles) * BN + half * MINE * 64, 0);
         }
         int t = 0;
-        // every epilogue warp walks every tile even after an abort (skipping the work), so that nobody
-        // is left waiting alone at the named barrier below
-        for (int w = first; w < n_work; w += stride, ++t) {
+        for (int w = first; ok && w < n_work; w += stride, ++t) {
             const int buf = t & 1, tile = w / p.slices;
             const int row0 = (tile / n_tiles) * C::TILE_M + (int)rank * BM + q * 32, n0 = (tile % n_tiles) * BN;
-            if (!p.out_f32) {
-                if (etid < BN) s->bias[buf][etid] = p.bias && n0 + etid < p.N ? load_any(p.bias, n0 + etid, p.bias_dtype) : 0.0f;
-                asm volatile("bar.sync 1, %0;" :: "n"(EPI_WARPS * 32) : "memory");
+            // the bias of this warp's columns, two a lane and piece, on its way while the tile's MMAs run.
+            // Each warp keeps its own copy: with one per tile, and a barrier for it, the warps waited for
+            // one another in a fifth of all cycles.
+            float bias_lo[MINE], bias_hi[MINE];
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) {
+                const int c = n0 + (half * MINE + i) * 64 + lane;
+                bias_lo[i] = p.bias && c < p.N ? load_any(p.bias, c, p.bias_dtype) : 0.0f;
+                bias_hi[i] = p.bias && c + 32 < p.N ? load_any(p.bias, c + 32, p.bias_dtype) : 0.0f;
             }
-            if (ahead && ok && MINE == 2 && lane == 0) {
+            if (ahead && MINE == 2 && lane == 0) {
                 // the second piece's residual as early as its buffer, which the last tile's second piece
                 // left through, is free; the first one's was asked for at the end of that tile
                 tma_wait_read<0>();
                 fetch_residual(row0, n0 + (half * MINE + 1) * 64, 1);
             }
-            if (ok) ok = wait_bar_warp<CG>(&s->acc_full[buf], full_phase[buf], s, 4, peer_abort);
-            if (!ok) continue;
+            ok = wait_bar_warp<CG>(&s->acc_full[buf], full_phase[buf], s, 4, peer_abort);
+            if (!ok) break;
             full_phase[buf] ^= 1;
             tc_fence_after();
             const uint32_t t_base = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * MINE * 64);
@@ -584,7 +587,10 @@ linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     if (p.tma_out && lane == 0) tma_wait_read<0>();
                     __syncwarp();
                 }
-                const float* const bias = s->bias[buf] + (half * MINE + i) * 64;
+                float* const bias = s->bias[ew];
+                bias[lane] = i == 0 ? bias_lo[0] : bias_lo[MINE - 1];
+                bias[lane + 32] = i == 0 ? bias_hi[0] : bias_hi[MINE - 1];
+                __syncwarp();
 #pragma unroll
                 for (int v = 0; v < 8; ++v) {
                     const ulonglong2 b0 = *reinterpret_cast<const ulonglong2*>(bias + v * 8), b1 = *reinterpret_cast<const ulonglong2*>(bias + v * 8 + 4);
