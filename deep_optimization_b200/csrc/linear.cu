@@ -557,7 +557,7 @@ extern "C" int act_linear_bwd(const void* dz, int64_t ld_dz, const void* x, int6
 }
 
 namespace {
-// slices of the rows for the column sums: about four blocks per SM
+// slices of the rows for the column sums: about six blocks per SM
 void mul_grid(int64_t M, int N, bool vec, int& tpr, int& gx, int& gy) {
     const int v = vec ? 8 : 1;
     const int64_t vecs = ceil_div(N, v);
@@ -567,6 +567,8 @@ void mul_grid(int64_t M, int N, bool vec, int& tpr, int& gx, int& gy) {
     int64_t want = ceil_div(act::stream_grid_for((int64_t)1 << 40, 6, 1), gx);
     const int64_t most = ceil_div(M, (int64_t)rpi * 4);
     if (want > most) want = most;
+    // up to four steps of the block: one slice, whose sums are the result, and no second launch
+    if (most <= 4) want = 1;
     gy = (int)(want < 1 ? 1 : (want > 65535 ? 65535 : want));
 }
 bool mul_vec(const void* dy, const void* d, const void* dz, int N) {
@@ -580,7 +582,8 @@ extern "C" size_t act_mul_col_sum_workspace(int64_t M, int N)
     int tpr, gx, gy, gy1;
     mul_grid(M, N, false, tpr, gx, gy);
     mul_grid(M, N, true, tpr, gx, gy1);
-    return (size_t)(gy > gy1 ? gy : gy1) * (size_t)N * 4;
+    if (gy < gy1) gy = gy1;
+    return gy == 1 ? 0 : (size_t)gy * (size_t)N * 4;
 }
 
 extern "C" int act_mul_col_sum(const void* dy, const void* d, int dtype, int64_t M, int N, void* dz, float* db,
@@ -597,19 +600,20 @@ extern "C" int act_mul_col_sum(const void* dy, const void* d, int dtype, int64_t
     if (!dy || !d || !dz) return ACT_ERR_NULL;
     if (((uintptr_t)dy | (uintptr_t)d | (uintptr_t)dz) & 1) return ACT_ERR_ALIGN;
     if (((uintptr_t)db | (db ? (uintptr_t)workspace : 0)) & 3) return ACT_ERR_ALIGN;
-    if (db && (!workspace || ws_bytes < act_mul_col_sum_workspace(M, N))) return ACT_ERR_WORKSPACE;
+    const size_t need = db ? act_mul_col_sum_workspace(M, N) : 0;
+    if (need && (!workspace || ws_bytes < need)) return ACT_ERR_WORKSPACE;
     const bool vec = mul_vec(dy, d, dz, N);
     int tpr, gx, gy;
     mul_grid(M, N, vec, tpr, gx, gy);
     const auto* a = static_cast<const unsigned short*>(dy);
     const auto* b = static_cast<const unsigned short*>(d);
     auto* o = static_cast<unsigned short*>(dz);
-    float* part = db ? static_cast<float*>(workspace) : nullptr;
+    float* part = !db ? nullptr : (gy == 1 ? db : static_cast<float*>(workspace));
     const dim3 grid((unsigned)gx, (unsigned)gy);
     if (vec) mul_col_sum_kernel<4><<<grid, kMulThreads, 0, st>>>(a, b, o, part, M, N, dtype, tpr);
     else mul_col_sum_kernel<0><<<grid, kMulThreads, 0, st>>>(a, b, o, part, M, N, dtype, tpr);
     if (cudaGetLastError() != cudaSuccess) return ACT_ERR_LAUNCH;
-    if (db) {
+    if (db && gy > 1) {
         col_sum_slices_kernel<<<(unsigned)ceil_div(N, 32), 1024, 0, st>>>(part, gy, N, db);
         if (cudaGetLastError() != cudaSuccess) return ACT_ERR_LAUNCH;
     }

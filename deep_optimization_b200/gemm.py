@@ -224,8 +224,9 @@ def act_backward(dy: torch.Tensor, derivative: torch.Tensor, bias_grad: bool = T
             db = torch.empty(N, dtype=torch.float32, device=dy.device)
             db_ptr = db.data_ptr()
             need = lib.act_mul_col_sum_workspace(M, N)
-            workspace = torch.empty(need, dtype=torch.uint8, device=dy.device)
-            ws_ptr = workspace.data_ptr()
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=dy.device)
+                ws_ptr = workspace.data_ptr()
         rc = lib.act_mul_col_sum(dy.data_ptr(), derivative.data_ptr(), _DTYPE16[dy.dtype], M, N, dz.data_ptr(), db_ptr, ws_ptr,
                                  need, _lib.stream_ptr(dy))
     _lib.check(rc, "act_mul_col_sum")

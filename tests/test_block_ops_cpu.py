@@ -87,7 +87,8 @@ def test_mul_col_sum_refusals(lib):
     assert f(None, P, 1, 4, 8, P, P, P, 1 << 20, None) == NULL
     assert f(ODD, P, 1, 4, 8, P, P, P, 1 << 20, None) == ALIGN
     assert f(P, P, 1, 4, 8, P, ctypes.c_void_p(4098), P, 1 << 20, None) == ALIGN
-    assert f(P, P, 1, 4, 8, P, P, None, 0, None) == WORKSPACE
+    assert f(P, P, 1, 40000, 8, P, P, None, 0, None) == WORKSPACE
+    assert lib.act_mul_col_sum_workspace(4, 8) == 0 and lib.act_mul_col_sum_workspace(0, 8) == 0
     assert f(P, P, 1, 4, 0, P, P, None, 0, None) == 0
 
 

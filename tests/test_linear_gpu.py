@@ -177,7 +177,7 @@ def _mul_case(M, N, dtype, dev, seed=0):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("shape", [(1, 1), (1, 8), (3, 7), (1003, 997), (5000, 768), (40, 4096), (9, 2056), (20000, 64), (333, 3001)])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 8), (3, 7), (1003, 997), (5000, 768), (40, 4096), (9, 2056), (20000, 64), (333, 3001), (16, 2048), (17, 2048), (16, 2049), (17, 301)])
 def test_act_backward(cuda_device, dtype, shape):
     _mul_case(*shape, dtype, cuda_device)
 
