@@ -20,7 +20,7 @@ from torch.nn.modules.utils import _pair, _single, _triple
 
 from .. import codec
 from ..gemm import act_backward, dw_from_packed, linear_act, linear_backward
-from .module_utils import low_pass_upsampled, unified_dequantize, unified_quantize
+from .module_utils import ChannelsLastShape, low_pass_upsampled, unified_dequantize, unified_quantize
 
 
 def _patchify_applies(input, weight, stride, padding, dilation, groups) -> bool:
@@ -259,6 +259,13 @@ class _DOLinear(Function):
         return dx, dw, None, None, None, None, db
 
 
+def _flat_groups(q_meta) -> bool:
+    """Whole groups over the tensor as it lies in memory: no padding, tiling or averaging."""
+    (bits, pack_only, _gs, act_padding, _N, _G, _h, _w, pad_elig, reshape_elig, _cm, avg_alam, _ab, shape) = q_meta
+    return (not pack_only and not act_padding and not pad_elig and not reshape_elig and not avg_alam
+            and bits in (1, 2, 4, 8) and not isinstance(shape, ChannelsLastShape))
+
+
 class _DOLinearAct(Function):
     """f(x W^T + b) + residual with the bias, the activation and the residual in the product's epilogue
     (`gemm.linear_act`; an extension: the reference runs them as separate operators around F.linear,
@@ -290,6 +297,7 @@ class _DOLinearAct(Function):
             x_saved = (None, None, None)
         elif meta is not None:
             x_saved, ctx.x_meta, _ = unified_quantize(input, None, target_name, meta, clamp=True, clamp_alpha=clamp_alpha)
+        del out
         if d is not None and meta is not None:
             d_saved, ctx.d_meta, _ = unified_quantize(d, None, act_name, meta, clamp=False, clamp_alpha=0.0)
         ctx.save_for_backward(weight, *x_saved, *d_saved, sign)
@@ -304,14 +312,22 @@ class _DOLinearAct(Function):
         dres = dy if ctx.needs[4] else None
         if not (need_dx or need_dw or need_db):
             return None, None, None, None, dres, None, None, None, None
+        dz = None
         if sign is not None:
             d = (sign > 0).to(dy.dtype)
         elif ctx.d_meta is not None:
-            d = unified_dequantize((d, d_scale, d_min), ctx.d_meta, None).to(dy.dtype)
+            if _flat_groups(ctx.d_meta) and d_scale.dtype == torch.float32:
+                # decoded in the multiplication's own pass, not written out
+                dyc = dy.contiguous()
+                dyc = dyc.clone() if dyc.data_ptr() % 16 else dyc
+                dz = codec.mul_dequant_unpack(d, d_scale, d_min, dyc, ctx.d_meta[0], ctx.d_meta[2])
+                d = None
+            else:
+                d = unified_dequantize((d, d_scale, d_min), ctx.d_meta, None).to(dy.dtype)
         if d is not None:
             dz, db = act_backward(dy, d, bias_grad=need_db)
         else:
-            dz = dy.contiguous()
+            dz = dy.contiguous() if dz is None else dz
             db = dz.reshape(-1, dz.shape[-1])
             db = None if not need_db else codec.col_sum(db) if codec.col_sum_applies(db) else db.sum(0, dtype=torch.float32)
         wd, bd = ctx.dtypes

@@ -261,6 +261,35 @@ def test_controller_fuses_the_mlp(cuda_device, rotary):
         assert torch.isfinite(c.traced_model(x)).all()
 
 
+@pytest.mark.parametrize("features", [256, 200])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_linear_act_compressed_gradients(cuda_device, features, offset):
+    """DOLinearAct with a meta: 8-bit x and f', whole groups (256 features) or padded ones (200), against the
+    gradients of the same layer without: a stored value is off by less than a step of its group, range / 255,
+    at most 12 / 255 of x and 1.3 / 255 of f', as independent errors; bf16 roundings as above."""
+    from deep_optimization_b200.controller import find_group_size
+    from deep_optimization_b200.layers import DOLinearAct
+    torch.manual_seed(9)
+    meta = {}
+    for name, f in (("lin", 128), ("act", features)):
+        gs, pad = find_group_size(40 * f, 8)
+        meta[name] = {"pack_only": False, "bits": 8, "group_size": gs, "act_padding": pad, "N": 48, "AVG_ALAM": False,
+                      "ALAM_BITS": 0, "DIVISION": None}
+    m = DOLinearAct(128, features, "gelu").to(cuda_device, torch.bfloat16).train()
+    x = torch.randn(48, 40, 128, device=cuda_device).bfloat16().requires_grad_()
+    flat = torch.randn(48 * 40 * features + 8, device=cuda_device).bfloat16()
+    dy = flat[offset:offset + 48 * 40 * features].view(48, 40, features)      # one element off: not 16-byte aligned
+    wrt = [x, m.weight, m.bias]
+    want = torch.autograd.grad(m(x), wrt, dy)
+    m.meta, m.target_name, m.act_name = meta, "lin", "act"
+    got = torch.autograd.grad(m(x), wrt, dy)
+    eps = 2.0 ** -9
+    # f' has a root mean square of at least 0.5, x of 1: relative errors of a stored value, then the roundings
+    err_d, err_x = 1.3 / 255 / 0.5, 12.0 / 255
+    for a, b, e in zip(got, want, (err_d, err_d + err_x, err_d)):
+        assert (a.double() - b.double()).norm() <= (e + 6 * eps) * b.double().norm()
+
+
 def test_controller_with_everything(cuda_device):
     torch.manual_seed(7)
     c = _controlled(_vit(rotary=True, dropout=0.1), cuda_device, fuse_linear_act=True, compress_dropout=True)
